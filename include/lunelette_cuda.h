@@ -180,6 +180,113 @@ size_t lunelette_cuda_batch_free_positions(const lunelette_cuda_batch *batch);
 int lunelette_cuda_kv_copy(float *kv_pool, size_t num_pages, size_t layers, const int *src_pages,
     const int *dst_pages, size_t pairs, size_t last_slots, void *stream);
 
+/* ---------------- serving from a 4-bit KV cache */
+
+/* Element types of the rows that the functions below take and write. */
+enum { LUNELETTE_CUDA_FLOAT32 = 0, LUNELETTE_CUDA_BFLOAT16 = 1, LUNELETTE_CUDA_FLOAT16 = 2 };
+
+/* A paged cache that holds keys and values in 4.5 bits each: the FP32 pool of
+ * the functions above in a seventh of its bytes, for any number of KV heads
+ * (1..256) of 64 or 128 dims. `pool` is device memory of
+ * lunelette_cuda_kv4_bytes() bytes, 16-byte aligned; pages hold 64 positions.
+ *
+ * A row is quantised in groups of 32 dims. With m the group's value of largest
+ * magnitude (the positive one when both signs reach it), d = m / -8 is rounded
+ * to 8 significant bits (and to multiples of 2^-24, at most 8160 in magnitude)
+ * and stored as FP16; a value r is stored as the code
+ * c = clamp(round(r / d), -8, 7) + 8 and reads back as d * (c - 8), which FP16
+ * holds exactly. Roundings go to the nearest, ties to even, and are decided as
+ * in 64-bit arithmetic. A group of zeros, or of values too small for the grid,
+ * reads back as zeros, and one that holds a NaN or an infinity as NaNs.
+ *
+ * [layer][page][KV head] is a block of K codes, K scales, V codes, V scales.
+ * Eight consecutive dims make a 32-bit word, the first dim in the lowest bits.
+ * Word 4 j + t (group j) of a K row is stored as word t * (head_dim / 32) + j of
+ * the row; V word n of a block, counted over its 64 rows, as word
+ * n ^ 8 * ((n >> 5) & m), m = 3 for 128 dims and 1 for 64. K scales lie
+ * [position][group], V scales [position / 2][group][position % 2]. */
+typedef struct lunelette_cuda_kv4 {
+    void *pool;
+    size_t layers, pages, kv_heads, head_dim;
+} lunelette_cuda_kv4;
+
+/* Bytes of a pool of these sizes; 0 when they are not supported. */
+size_t lunelette_cuda_kv4_bytes(size_t layers, size_t pages, size_t kv_heads, size_t head_dim);
+
+/* The rows of one call over several sequences. Row offsets[s] + i is row i of
+ * sequence s, n = offsets[s + 1] - offsets[s] rows in all, at position
+ * lengths[s] - n + i: lengths counts the positions that the sequence holds with
+ * this call's rows. Position p lives in page page_tables[s * table_stride +
+ * p / 64], slot p % 64. The three arrays are device memory, read when the call
+ * runs on its stream, so that a captured call follows later contents; the
+ * counts are bounds that the launch is sized by:
+ *   rows        rows of the tensors; those from offsets[sequences] on are left
+ *               as they are
+ *   max_count   at least every n
+ *   max_length  at least every length, at most table_stride * 64
+ * The functions that take a device word `status` (or NULL) OR 1 into it when a
+ * sequence breaks these bounds or its offsets descend (its rows are skipped and
+ * left as they are), and 2 when a page lies outside the pool (its positions are
+ * skipped). Sequences may be empty, and a row before position 0 (n > length)
+ * has no position: nothing is stored or read for it. Sequences of one call must
+ * not append to the same page. */
+typedef struct lunelette_cuda_rows {
+    size_t rows, sequences;
+    const int *offsets, *lengths, *page_tables;
+    size_t table_stride, max_count, max_length;
+} lunelette_cuda_rows;
+
+/* Append: row r of k and v (kv_heads * head_dim elements each, consecutive rows
+ * k_stride and v_stride elements apart) goes to its position of `layer`, the
+ * keys rotated on the way: dims j and j + head_dim / 2 by cos and sin of row
+ * `position` of the tables [rope_positions][head_dim] (as _qkv_rope; NULL: no
+ * rotation). Where q is given, its query_heads heads are rotated too, times the
+ * checkpoint's query scale 1 + 0.1 ln(1 + floor(position / 16384)) as
+ * _qkv_rope, into q_out (which may be q). `type` is that of k, v, q and q_out. Rows of k and v
+ * may be slices of one projection's output. The reference's counterpart is the
+ * KV blit behind its rope kernel (src/metal_encode.m:129-153). */
+int lunelette_cuda_kv4_append(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,
+    int type, const void *k, size_t k_stride, const void *v, size_t v_stride, const void *q, size_t q_stride,
+    size_t query_heads, void *q_out, size_t q_out_stride, const float *rope_cos, const float *rope_sin,
+    size_t rope_positions, int *status, void *stream);
+
+/* Read rows back: the values that the cache holds at each row's position, into
+ * rows of k and v (either may be NULL) of `type`. Lengths and offsets may name
+ * any positions that were appended. */
+int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,
+    int type, void *k, size_t k_stride, void *v, size_t v_stride, int *status, void *stream);
+
+/* Causal attention over the cache: row r's query heads (query_heads a multiple
+ * of kv_heads, head h over KV head h / (query_heads / kv_heads)) see positions
+ * 0..its own of its sequence: out = sum_p softmax_p(scale * q . k_p) v_p, with
+ * scores, softmax and sums as in FP32. Rows without a position get zeros. q is
+ * rotated already and may not overlap out. `workspace` (16-byte aligned, no
+ * content expected or kept) holds at least
+ * lunelette_cuda_kv4_attention_workspace() bytes for the same sizes; calls that
+ * may overlap on the GPU, captured graphs among them, need one each. A
+ * deterministic result: the same call gives the same bits. */
+size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
+    size_t query_heads);
+int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,
+    int type, const void *q, size_t q_stride, size_t query_heads, float scale, void *out, size_t out_stride,
+    void *workspace, size_t workspace_bytes, int *status, void *stream);
+
+/* ---------------- probabilities from logits */
+
+/* For each row of logits [rows][vocab] (`type`, rows `stride` elements apart):
+ * logprobs[r], the log probability of token targets[r] (device; NaN for one
+ * outside 0..vocab-1), entropy[r] of the row in nats, and its `top` (0..64, at
+ * most vocab) most probable tokens, ids and log probabilities [rows][top] in
+ * falling order, ties to the lowest id. Any of the outputs may be NULL (targets
+ * and logprobs together, top_ids and top_logprobs together with top 0).
+ * Sums run in FP32. Logits of -infinity have probability 0; a row with a NaN, a
+ * +infinity or only -infinity has NaN probabilities and entropy, and its top
+ * ids are those of the largest logits with NaN above all. The device form of
+ * what callers compute from the logits that prefill, append and decode return. */
+int lunelette_cuda_token_logprobs(const void *logits, int type, size_t rows, size_t vocab, size_t stride,
+    const int64_t *targets, size_t top, float *logprobs, float *entropy, int64_t *top_ids, float *top_logprobs,
+    void *stream);
+
 /* ---------------- model-level test support */
 
 /* Keep every layer's output rows (which 0..25) and the final-norm rows (26) of

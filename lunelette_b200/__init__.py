@@ -42,10 +42,27 @@ class Memory(ctypes.Structure):
                 ("kv_bytes", ctypes.c_uint64), ("total_bytes", ctypes.c_uint64)]
 
 
+class Kv4(ctypes.Structure):
+    """lunelette_cuda_kv4: a paged 4-bit KV cache over a device pool."""
+    _fields_ = [("pool", ctypes.c_void_p), ("layers", ctypes.c_size_t), ("pages", ctypes.c_size_t),
+                ("kv_heads", ctypes.c_size_t), ("head_dim", ctypes.c_size_t)]
+
+
+class Rows(ctypes.Structure):
+    """lunelette_cuda_rows: the rows of one call over several sequences."""
+    _fields_ = [("rows", ctypes.c_size_t), ("sequences", ctypes.c_size_t), ("offsets", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("page_tables", ctypes.c_void_p), ("table_stride", ctypes.c_size_t),
+                ("max_count", ctypes.c_size_t), ("max_length", ctypes.c_size_t)]
+
+
+FLOAT32, BFLOAT16, FLOAT16 = 0, 1, 2
+
 _lib = None
 P = ctypes.c_void_p
 SZ = ctypes.c_size_t
 ERR = ctypes.c_char_p
+INT = ctypes.c_int
+CACHE, ROWS = ctypes.POINTER(Kv4), ctypes.POINTER(Rows)
 
 # name -> (restype, argtypes); every symbol include/metal.h and include/lunelette_cuda.h declare
 SIGNATURES = {
@@ -86,6 +103,12 @@ SIGNATURES = {
     "lunelette_cuda_head_bf16": (ctypes.c_int, [P, SZ, SZ, P, P, P, P, P]),
     "lunelette_cuda_attention": (ctypes.c_int, [P, P, P, SZ, SZ, SZ, SZ, P, P, P, SZ, P]),
     "lunelette_cuda_attention_noalloc": (ctypes.c_int, [P, P, P, SZ, SZ, SZ, SZ, P, P, ERR, SZ]),
+    "lunelette_cuda_kv4_bytes": (SZ, [SZ, SZ, SZ, SZ]),
+    "lunelette_cuda_kv4_append": (INT, [CACHE, SZ, ROWS, INT, P, SZ, P, SZ, P, SZ, SZ, P, SZ, P, P, SZ, P, P]),
+    "lunelette_cuda_kv4_read": (INT, [CACHE, SZ, ROWS, INT, P, SZ, P, SZ, P, P]),
+    "lunelette_cuda_kv4_attention_workspace": (SZ, [CACHE, ROWS, SZ]),
+    "lunelette_cuda_kv4_attention": (INT, [CACHE, SZ, ROWS, INT, P, SZ, SZ, ctypes.c_float, P, SZ, P, SZ, P, P]),
+    "lunelette_cuda_token_logprobs": (INT, [P, INT, SZ, SZ, SZ, P, SZ, P, P, P, P, P]),
     "lunelette_cuda_trace": (ctypes.c_int, [P, ctypes.c_int]),
     "lunelette_cuda_trace_copy": (ctypes.c_int, [P, ctypes.c_int, P, SZ]),
     "lunelette_cuda_snapshot": (P, [P, ctypes.c_int]),

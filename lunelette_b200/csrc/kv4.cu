@@ -1,0 +1,216 @@
+// C-ABI of the 4-bit KV cache (include/lunelette_cuda.h): argument checks and launches.
+#include "kv4_attention.cuh"
+#include "launch.h"
+
+#include "lunelette_cuda.h"
+
+#include <limits.h>
+#include <string.h>
+
+#define LUN_API extern "C" __attribute__((visibility("default")))
+
+using namespace lun;
+
+namespace {
+
+constexpr size_t kMaxRows = 1 << 24, kMaxLength = 1 << 28;
+
+bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+size_t element_size(int type) { return type == LUNELETTE_CUDA_FLOAT32 ? 4 : 2; }
+
+bool valid_type(int type)
+{
+    return type == LUNELETTE_CUDA_FLOAT32 || type == LUNELETTE_CUDA_BFLOAT16 || type == LUNELETTE_CUDA_FLOAT16;
+}
+
+size_t block_bytes(size_t head_dim) { return head_dim == 128 ? Kv4Layout<128>::block : Kv4Layout<64>::block; }
+
+bool valid_sizes(size_t layers, size_t pages, size_t kv_heads, size_t head_dim)
+{
+    return layers && layers <= 4096 && pages && pages <= INT_MAX / 64 && kv_heads && kv_heads <= 256 &&
+           (head_dim == 64 || head_dim == 128);
+}
+
+bool valid_cache(const lunelette_cuda_kv4 *c, size_t layer)
+{
+    return c && c->pool && aligned(c->pool, 16) && valid_sizes(c->layers, c->pages, c->kv_heads, c->head_dim) &&
+           layer < c->layers;
+}
+
+// The sizes of a call; `empty` when there is nothing to do.
+bool valid_rows(const lunelette_cuda_rows *r, bool *empty)
+{
+    if (!r) return false;
+    *empty = !r->rows || !r->sequences || !r->max_count;
+    if (r->rows > kMaxRows || r->sequences > kMaxRows || r->max_count > kMaxRows || r->max_length > kMaxLength)
+        return false;
+    if (r->table_stride > kMaxLength || r->max_length > r->table_stride * kPage || !aligned(r->offsets, 4) ||
+        !aligned(r->lengths, 4) || !aligned(r->page_tables, 4))
+        return false;
+    return *empty || (r->offsets && r->lengths && r->page_tables);
+}
+
+Kv4Cache cache_of(const lunelette_cuda_kv4 *c, size_t layer)
+{
+    Kv4Cache k;
+    k.layer = static_cast<uint8_t *>(c->pool) + layer * c->pages * c->kv_heads * block_bytes(c->head_dim);
+    k.pages = (int)c->pages;
+    k.heads = (int)c->kv_heads;
+    return k;
+}
+
+Kv4Rows rows_of(const lunelette_cuda_rows *r)
+{
+    Kv4Rows k;
+    k.rows = (int)r->rows;
+    k.sequences = (int)r->sequences;
+    k.offsets = r->offsets;
+    k.lengths = r->lengths;
+    k.page_tables = r->page_tables;
+    k.table_stride = r->table_stride;
+    k.max_count = (int)r->max_count;
+    k.max_length = (int)r->max_length;
+    return k;
+}
+
+// Rows of `width` elements at a base, `stride` elements apart: element-aligned,
+// and *wide is cleared unless each starts on 16 bytes. A call without rows needs
+// no base.
+bool valid_tensor(const void *base, size_t stride, size_t width, int type, bool empty, bool *wide)
+{
+    const size_t size = element_size(type);
+    if (!base) return empty;
+    if (!aligned(base, size) || stride < width || stride > (size_t)1 << 32) return false;
+    if (!aligned(base, 16) || stride * size % 16) *wide = false;
+    return true;
+}
+
+template <typename F> cudaError_t by_type(int type, F &&f)
+{
+    switch (type) {
+    case LUNELETTE_CUDA_FLOAT32: return f((float)0);
+    case LUNELETTE_CUDA_BFLOAT16: return f(__nv_bfloat16());
+    default: return f(__half());
+    }
+}
+
+int ok(cudaError_t e) { return e == cudaSuccess ? 0 : -1; }
+
+}  // namespace
+
+LUN_API size_t lunelette_cuda_kv4_bytes(size_t layers, size_t pages, size_t kv_heads, size_t head_dim)
+{
+    return valid_sizes(layers, pages, kv_heads, head_dim) ? layers * pages * kv_heads * block_bytes(head_dim) : 0;
+}
+
+LUN_API int lunelette_cuda_kv4_append(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,
+                                      int type, const void *k, size_t k_stride, const void *v, size_t v_stride,
+                                      const void *q, size_t q_stride, size_t query_heads, void *q_out,
+                                      size_t q_out_stride, const float *rope_cos, const float *rope_sin,
+                                      size_t rope_positions, int *status, void *stream)
+{
+    bool empty = false, wide = true;
+    if (!valid_cache(cache, layer) || !valid_rows(rows, &empty) || !valid_type(type)) return -1;
+    const size_t width = cache->kv_heads * cache->head_dim, q_width = query_heads * cache->head_dim;
+    if (!q != !q_out || !rope_cos != !rope_sin || (q && (!query_heads || query_heads > 4096))) return -1;
+    if (rope_cos && (!aligned(rope_cos, 16) || !aligned(rope_sin, 16) || rows->max_length > rope_positions)) return -1;
+    if (!valid_tensor(k, k_stride, width, type, empty, &wide) || !valid_tensor(v, v_stride, width, type, empty, &wide))
+        return -1;
+    if (q && (!valid_tensor(q, q_stride, q_width, type, empty, &wide) ||
+              !valid_tensor(q_out, q_out_stride, q_width, type, empty, &wide)))
+        return -1;
+    if (!aligned(status, 4)) return -1;
+    if (empty) return 0;
+    Kv4AppendParams p;
+    memset(&p, 0, sizeof p);
+    p.cache = cache_of(cache, layer);
+    p.rows = rows_of(rows);
+    p.k = k;
+    p.v = v;
+    p.q = q;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.q_stride = q_stride;
+    p.q_out = q_out;
+    p.q_out_stride = q_out_stride;
+    p.query_heads = q ? (int)query_heads : 0;
+    p.cosine = rope_cos;
+    p.sine = rope_sin;
+    p.wide = wide;
+    p.status = status;
+    return ok(by_type(type, [&](auto t) {
+        using T = decltype(t);
+        auto kernel = cache->head_dim == 128 ? kv4_append_kernel<128, T> : kv4_append_kernel<64, T>;
+        return launch(kernel, dim3((unsigned)rows->rows), dim3(256), 0, (cudaStream_t)stream, p);
+    }));
+}
+
+LUN_API int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,
+                                    int type, void *k, size_t k_stride, void *v, size_t v_stride, int *status,
+                                    void *stream)
+{
+    bool empty = false, wide = true;
+    if (!valid_cache(cache, layer) || !valid_rows(rows, &empty) || !valid_type(type)) return -1;
+    const size_t width = cache->kv_heads * cache->head_dim;
+    if (!valid_tensor(k, k_stride, width, type, true, &wide) || !valid_tensor(v, v_stride, width, type, true, &wide) ||
+        !aligned(status, 4))
+        return -1;
+    if (empty || (!k && !v)) return 0;
+    Kv4ReadParams p;
+    memset(&p, 0, sizeof p);
+    p.cache = cache_of(cache, layer);
+    p.rows = rows_of(rows);
+    p.k = k;
+    p.v = v;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.wide = wide;
+    p.status = status;
+    return ok(by_type(type, [&](auto t) {
+        using T = decltype(t);
+        auto kernel = cache->head_dim == 128 ? kv4_read_kernel<128, T> : kv4_read_kernel<64, T>;
+        return launch(kernel, dim3((unsigned)rows->rows), dim3(256), 0, (cudaStream_t)stream, p);
+    }));
+}
+
+LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
+                                                      size_t query_heads)
+{
+    (void)cache, (void)rows, (void)query_heads;
+    return 0;
+}
+
+LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer,
+                                         const lunelette_cuda_rows *rows, int type, const void *q, size_t q_stride,
+                                         size_t query_heads, float scale, void *out, size_t out_stride,
+                                         void *workspace, size_t workspace_bytes, int *status, void *stream)
+{
+    bool empty = false, wide = true;
+    if (!valid_cache(cache, layer) || !valid_rows(rows, &empty) || !valid_type(type)) return -1;
+    if (!query_heads || query_heads > 4096 || query_heads % cache->kv_heads || !(scale - scale == 0.0f)) return -1;
+    if (workspace_bytes < lunelette_cuda_kv4_attention_workspace(cache, rows, query_heads) || !aligned(workspace, 16))
+        return -1;
+    const size_t width = query_heads * cache->head_dim;
+    if (!valid_tensor(q, q_stride, width, type, empty, &wide) ||
+        !valid_tensor(out, out_stride, width, type, empty, &wide) || !aligned(status, 4))
+        return -1;
+    if (empty) return 0;
+    Kv4AttnParams p;
+    memset(&p, 0, sizeof p);
+    p.cache = cache_of(cache, layer);
+    p.rows = rows_of(rows);
+    p.q = q;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.query_heads = (int)query_heads;
+    p.group = (int)(query_heads / cache->kv_heads);
+    p.scale = scale;
+    p.status = status;
+    return ok(by_type(type, [&](auto t) {
+        using T = decltype(t);
+        auto kernel = cache->head_dim == 128 ? kv4_attention_kernel<128, T> : kv4_attention_kernel<64, T>;
+        return launch(kernel, dim3((unsigned)rows->rows, (unsigned)query_heads), dim3(32), 0, (cudaStream_t)stream, p);
+    }));
+}
