@@ -174,11 +174,51 @@ LUN_API int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t laye
     }));
 }
 
+// How a call's keys and rows are split over the GPU.
+struct AttnPlan {
+    int nt, tile_rows, tiles, split_pages, splits;
+    size_t part_bytes;
+};
+
+static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows, size_t query_heads)
+{
+    AttnPlan a;
+    const size_t group = query_heads / cache->kv_heads, most = rows->max_count * group;
+    a.nt = most <= 4 ? 1 : 2;
+    a.tile_rows = 4 * a.nt;
+    a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
+    const size_t pages = (rows->max_length + kPage - 1) / kPage;
+    const size_t items = rows->sequences * cache->kv_heads * a.tiles;
+    size_t per = pages * items / (2 * 148);
+    per = per < 4 ? 4 : per > 64 ? 64 : per;
+    a.split_pages = (int)((per + 3) / 4 * 4);
+    a.splits = (int)((pages + a.split_pages - 1) / a.split_pages);
+    if (a.splits < 1) a.splits = 1;
+    a.part_bytes = a.splits == 1 ? 0 : items * a.tile_rows * a.splits * (cache->head_dim + 2) * sizeof(float);
+    return a;
+}
+
 LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
                                                       size_t query_heads)
 {
-    (void)cache, (void)rows, (void)query_heads;
-    return 0;
+    bool empty = false;
+    if (!valid_cache(cache, 0) || !valid_rows(rows, &empty) || !query_heads || query_heads > 4096 ||
+        query_heads % cache->kv_heads || empty)
+        return 0;
+    return plan_attention(cache, rows, query_heads).part_bytes;
+}
+
+template <int D, typename T, int NT>
+static cudaError_t launch_decode(const Kv4AttnParams &p, const AttnPlan &a, int sequences, cudaStream_t stream)
+{
+    constexpr int smem = Kv4Decode<D, NT>::smem;
+    auto kernel = kv4_decode_kernel<D, T, NT>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const size_t items = (size_t)sequences * p.cache.heads * a.tiles;
+    e = launch(kernel, dim3((unsigned)(items * a.splits)), dim3(32 * kDecodeWarps), smem, stream, p);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * a.nt)), dim3(128), 0, stream, p, a.tiles * a.tile_rows);
 }
 
 LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer,
@@ -189,13 +229,14 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
     bool empty = false, wide = true;
     if (!valid_cache(cache, layer) || !valid_rows(rows, &empty) || !valid_type(type)) return -1;
     if (!query_heads || query_heads > 4096 || query_heads % cache->kv_heads || !(scale - scale == 0.0f)) return -1;
-    if (workspace_bytes < lunelette_cuda_kv4_attention_workspace(cache, rows, query_heads) || !aligned(workspace, 16))
-        return -1;
     const size_t width = query_heads * cache->head_dim;
     if (!valid_tensor(q, q_stride, width, type, empty, &wide) ||
-        !valid_tensor(out, out_stride, width, type, empty, &wide) || !aligned(status, 4))
+        !valid_tensor(out, out_stride, width, type, empty, &wide) || !aligned(status, 4) || !aligned(workspace, 16))
         return -1;
     if (empty) return 0;
+    const AttnPlan a = plan_attention(cache, rows, query_heads);
+    if (workspace_bytes < a.part_bytes || (a.part_bytes && !workspace)) return -1;
+    if (rows->sequences * cache->kv_heads * a.tiles > (size_t)INT_MAX / a.splits) return -1;
     Kv4AttnParams p;
     memset(&p, 0, sizeof p);
     p.cache = cache_of(cache, layer);
@@ -204,13 +245,20 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
     p.out = out;
     p.q_stride = q_stride;
     p.out_stride = out_stride;
-    p.query_heads = (int)query_heads;
     p.group = (int)(query_heads / cache->kv_heads);
-    p.scale = scale;
+    p.scale2 = scale * 1.4426950408889634f;
+    p.split_pages = a.split_pages;
+    p.splits = a.splits;
+    p.tiles = a.tiles;
+    p.wide = wide;
+    p.part = static_cast<float *>(workspace);
     p.status = status;
+    const int sequences = (int)rows->sequences;
+    cudaStream_t st = (cudaStream_t)stream;
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
-        auto kernel = cache->head_dim == 128 ? kv4_attention_kernel<128, T> : kv4_attention_kernel<64, T>;
-        return launch(kernel, dim3((unsigned)rows->rows, (unsigned)query_heads), dim3(32), 0, (cudaStream_t)stream, p);
+        if (cache->head_dim == 128)
+            return a.nt == 1 ? launch_decode<128, T, 1>(p, a, sequences, st) : launch_decode<128, T, 2>(p, a, sequences, st);
+        return a.nt == 1 ? launch_decode<64, T, 1>(p, a, sequences, st) : launch_decode<64, T, 2>(p, a, sequences, st);
     }));
 }

@@ -1,8 +1,33 @@
-// Causal attention over the paged 4-bit KV cache.
+// Causal attention over the paged 4-bit KV cache for few query rows: decode
+// steps over many sequences, and short runs of tokens.
+//
+// HBM-bound by design: a block of the cache (one page of one KV head, K and V with their
+// scales, 9216 bytes for 128 dims) is copied once into shared memory by one bulk
+// copy and serves all the query rows of its KV head. Each warp walks pages of its
+// own with its own ring of blocks, so nothing waits for another warp until the
+// last merge; keys split over warps, CTAs (splits) and, in the combine kernel,
+// back together in a fixed order.
+//
+// The products run on mma.sync m16n8k16 with FP16 operands and FP32 sums: a
+// decode step has 1 to 8 query rows a KV head, so a tcgen05 tile of 128 rows would be
+// 94% padding, while here the rows sit in the n = 8 side. FP32 rows of q and
+// weights of the softmax enter as FP16 hi + lo parts in neighbouring columns
+// (22 bits together), so one MMA serves 4 rows at FP32 grade.
+//   S = K Q^T     A: 16 keys x 16 dims of integers c - 8 straight from the
+//                 codes (exact); a group's sum is scaled by d in FP32 after its
+//                 two MMAs, so K needs no multiplication per element.
+//   O^T = V^T P^T A: 16 dims x 16 keys of d * (c - 8), exact in FP16; B: the
+//                 weights, moved from S's layout by movmatrix.
+// A code becomes FP16 by OR-ing it into the mantissa of 1024 (low nibble of a
+// byte) or of 1024 scaled by 16 (high nibble) and subtracting: both exact.
 #pragma once
+#include "async.cuh"
+#include "attention.cuh"
 #include "kv4.cuh"
 
 namespace lun {
+
+constexpr int kKv4Timeout = 4;  // status bit: a bounded wait gave up, outputs are not valid
 
 struct Kv4AttnParams {
     Kv4Cache cache;
@@ -10,71 +35,432 @@ struct Kv4AttnParams {
     const void *q;
     void *out;
     size_t q_stride, out_stride;
-    int query_heads, group;
-    float scale;
+    int group;        // query heads per KV head
+    float scale2;     // scale * log2 e
+    int split_pages;  // pages of a split
+    int splits;       // 1: the kernel writes the output itself
+    int tiles;        // row tiles of a (sequence, KV head)
+    bool wide;
+    float *part;      // [sequence][KV head][row of the tiles][split][D + 2]: unnormalised o, m, l
     int *status;
 };
 
-// One warp per (row, query head), 32 keys a step: a lane scores one key, then
-// takes D / 32 dims of the weighted sum.
-template <int D, typename T>
-static __global__ void __launch_bounds__(32) kv4_attention_kernel(Kv4AttnParams p)
+static __device__ int kv4_error_sink;
+
+// The softmax's weights are taken times 2^14, and l with them: the largest is
+// 16384, and the FP16 parts of a weight keep 22 bits down to 2^-28 of it, where a
+// largest weight of 1 would leave small ones on the 2^-24 grid of FP16's
+// subnormals.
+constexpr float kWeightShift = 14.0f;
+
+constexpr int kDecodeWarps = 4, kDecodeStages = 3;
+
+template <int D, int NT> struct Kv4Decode {
+    static constexpr int rows = 4 * NT;  // query rows of a tile
+    static constexpr int ring = kDecodeWarps * kDecodeStages * Kv4Layout<D>::block;
+    static constexpr int merge = kDecodeWarps * rows * (D + 2) * 4;
+    static constexpr int smem = 128 + (ring > merge ? ring : merge) + kDecodeWarps * kDecodeStages * 8 + 16;
+};
+
+// Four codes in the bytes' low and high nibbles of both halves -> c - 8 in FP16:
+// a = (nibble 0, nibble 4), b = (nibble 1, nibble 5) of a word.
+__device__ __forceinline__ uint32_t kv4_low(uint32_t w)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+    const __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&r), __half2half2(__ushort_as_half(0x6408)));  // 1032
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t kv4_high(uint32_t w)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+    // (1024 + 16 c) / 16 - 72
+    const __half2 h = __hfma2(*reinterpret_cast<__half2 *>(&r), __half2half2(__ushort_as_half(0x2c00)),
+                              __half2half2(__ushort_as_half(0xd480)));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t kv4_times(uint32_t v, uint32_t d)
+{
+    const __half2 h = __hmul2(*reinterpret_cast<__half2 *>(&v), *reinterpret_cast<__half2 *>(&d));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float low_half(uint32_t v) { return __low2float(*reinterpret_cast<__half2 *>(&v)); }
+__device__ __forceinline__ float high_half(uint32_t v) { return __high2float(*reinterpret_cast<__half2 *>(&v)); }
+
+// 2^-e with 2^e the power of two at or below x's magnitude, e within +-120;
+// 1 for zero, NaN and infinities.
+__device__ __forceinline__ float power_scale(float x, float &back)
+{
+    int e = (int)(__float_as_uint(x) >> 23 & 255) - 127;
+    if (x == 0.0f || e == 128) e = 0;
+    e = max(-120, min(120, e));
+    back = __uint_as_float((uint32_t)(127 + e) << 23);
+    return __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// A block per (sequence, KV head, row tile, split), the split fastest.
+template <int D, typename T, int NT>
+static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv4AttnParams p)
 {
     using L = Kv4Layout<D>;
-    constexpr int per = D / 32;
-    const int row = blockIdx.x, head = blockIdx.y, kvh = head / p.group, lane = threadIdx.x;
-    __shared__ float qs[D];
+    using K = Kv4Decode<D, NT>;
+    constexpr int G = L::groups, MT = D / 16;  // m tiles of V's dims
+    extern __shared__ __align__(128) uint8_t kv4_smem[];
+    uint8_t *ring = kv4_smem;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(kv4_smem + K::smem - kDecodeWarps * kDecodeStages * 8 - 16);
+    volatile int *abort_word = reinterpret_cast<volatile int *>(bars + kDecodeWarps * kDecodeStages);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % p.splits, tile_of = blockIdx.x / p.splits, r0 = tile_of % p.tiles * K::rows;
+    const int kvh = tile_of / p.tiles % p.cache.heads, s = tile_of / p.tiles / p.cache.heads;
     pdl_wait();
     pdl_launch_dependents();
-    const int s = kv4_sequence_of_row(p.rows, row);
     const Kv4Sequence q = kv4_sequence(p.rows, s);
     if (!q.ok) {
-        if (lane == 0) kv4_report(p.status, kKv4BadRows);
+        if (threadIdx.x == 0) kv4_report(p.status, kKv4BadRows);
         return;
     }
-    if (row < q.first || row >= q.first + q.count) return;
-    const int position = q.length - q.count + (row - q.first);
-    const T *src = static_cast<const T *>(p.q) + (size_t)row * p.q_stride + (size_t)head * D;
-    for (int d = lane; d < D; d += 32) qs[d] = to_float(src[d]) * p.scale;
-    __syncwarp();
-    float m = -INFINITY, l = 0.0f, o[per] = {};
+    const int n_rows = q.count * p.group;
+    if (r0 >= n_rows) return;
+    const int pages = (q.length + kPage - 1) / kPage, first = split * p.split_pages;
+    const int last = min(first + p.split_pages, pages);  // this split's pages [first, last)
+    if (first >= last && (split > 0 || p.splits > 1)) return;  // the combine knows how many splits have pages
+    if (threadIdx.x == 0) *abort_word = 0;
+    if (lane < kDecodeStages) mbar_init(&bars[warp * kDecodeStages + lane], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+
+    // the warp's pages are first + warp + 4 i; their ids, 32 at a time, one a lane
     const int *table = p.rows.page_tables + s * p.rows.table_stride;
-    for (int p0 = 0; p0 <= position; p0 += 32) {
-        const uint8_t *block = kv4_block<D>(p.cache, table[p0 / kPage], kvh);
-        if (!block) {
-            if (lane == 0) kv4_report(p.status, kKv4BadPage);
-            continue;
+    const int mine = last - first - warp > 0 ? (last - first - warp + kDecodeWarps - 1) / kDecodeWarps : 0;
+    uint8_t *buffers = ring + warp * kDecodeStages * L::block;
+    uint64_t *bar = bars + warp * kDecodeStages;
+    int ids = lane < mine ? table[first + warp + lane * kDecodeWarps] : 0;
+    int next_ids = 0;
+    auto id_of = [&](int i) { return __shfl_sync(0xffffffffu, (i & 32) ? next_ids : ids, i & 31); };
+    auto issue = [&](int i, int id) {
+        const uint8_t *block = kv4_block<D>(p.cache, id, kvh);
+        if (lane == 0 && block) {
+            mbar_expect_tx(&bar[i % kDecodeStages], L::block);
+            bulk_g2s(buffers + i % kDecodeStages * L::block, block, L::block, &bar[i % kDecodeStages]);
         }
-        const int slot = p0 % kPage + lane;
-        float score = -INFINITY;
-        if (p0 + lane <= position) {
-            score = 0.0f;
-            for (int w = 0; w < L::words; w++) {
-                const uint32_t word = *reinterpret_cast<const uint32_t *>(block + L::k_word(slot, w));
-                const float d = __half2float(*reinterpret_cast<const __half *>(block + L::k_scale(slot, w / 4)));
-                float sum = 0.0f;
-                for (int e = 0; e < 8; e++) sum = fmaf((float)((int)(word >> (4 * e) & 15u) - 8), qs[8 * w + e], sum);
-                score = fmaf(d, sum, score);
+    };
+    // q: two columns (hi, lo) a row; column g belongs to row g / 2
+    uint32_t qb[NT][D / 16][2];
+    float back[NT];  // what a score is multiplied with, of row nt * 4 + t
+    int limit[NT];   // that row's last visible position
+    for (int i = 0; i < kDecodeStages && i < mine; i++) issue(i, id_of(i));
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = r0 + 4 * nt + (g >> 1);
+        const bool live = r < n_rows;
+        const int token = live ? r / p.group : 0, head = kvh * p.group + (live ? r - token * p.group : 0);
+        const T *src = static_cast<const T *>(p.q) + (size_t)(q.first + token) * p.q_stride + (size_t)head * D + 8 * t;
+        float x[G][8], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            load8(src + 32 * j, p.wide, x[j]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (!live) x[j][e] = 0.0f;
+                top = fmaxf(top, fabsf(x[j][e]));
             }
         }
-        const float mx = fmaxf(m, warp_max(score));
-        const float corr = m == -INFINITY ? 0.0f : expf(m - mx);
-        const float prob = score == -INFINITY ? 0.0f : expf(score - mx);
-        m = mx;
-        l = l * corr + warp_sum(prob);
-        for (int e = 0; e < per; e++) o[e] *= corr;
-        for (int j = 0; j < 32 && p0 + j <= position; j++) {
-            const float pj = __shfl_sync(0xffffffffu, prob, j);
-            for (int e = 0; e < per; e++) {
-                const int d = lane * per + e, sl = p0 % kPage + j;
-                const uint32_t word = *reinterpret_cast<const uint32_t *>(block + L::v_word(sl, d / 8));
-                const float sc = __half2float(*reinterpret_cast<const __half *>(block + L::v_scale(sl, d / 32)));
-                o[e] = fmaf(pj, sc * (float)((int)(word >> (4 * (d % 8)) & 15u) - 8), o[e]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        float undo;
+        const float f = power_scale(top, undo);
+        // lane (g, t) scores row 4 nt + t, whose factors sit in lane (2 t, .)
+        back[nt] = __shfl_sync(0xffffffffu, undo, 8 * t) * p.scale2;
+#pragma unroll
+        for (int j = 0; j < G; j++)
+#pragma unroll
+            for (int hw = 0; hw < 2; hw++)
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    uint32_t hi, lo;
+                    split_half2(x[j][2 * hw + b] * f, x[j][2 * hw + b + 4] * f, hi, lo);
+                    qb[nt][2 * j + hw][b] = g & 1 ? lo : hi;
+                }
+        const int mine_r = r0 + 4 * nt + t;
+        limit[nt] = mine_r < n_rows ? q.length - q.count + mine_r / p.group : -1;
+    }
+    float m[NT], l[NT], o[NT][MT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MT; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+    }
+    bool ok = true;
+    unsigned phases = 0;  // parity of each stage's next wait
+    for (int i = 0; i < mine; i++) {
+        if ((i & 31) == 0 && i + 32 < mine) {  // the other half of the ids, long before it is asked for
+            const int fetched = i + 32 + lane < mine ? table[first + warp + (i + 32 + lane) * kDecodeWarps] : 0;
+            if (i & 32) ids = fetched;
+            else next_ids = fetched;
+        }
+        const int stage = i % kDecodeStages, page_index = first + warp + i * kDecodeWarps;
+        const int id = id_of(i);
+        if ((unsigned)id >= (unsigned)p.cache.pages) {
+            if (lane == 0) kv4_report(p.status, kKv4BadPage);
+        } else {
+            ok = warp_wait(&bar[stage], phases >> stage & 1, abort_word, &kv4_error_sink);
+            if (!ok) break;
+            phases ^= 1u << stage;
+            const uint8_t *block = buffers + stage * L::block;
+            const int p0 = page_index * kPage;
+            float sc[4][NT][2];
+#pragma unroll
+            for (int tile = 0; tile < 4; tile++) {
+                float acc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+                uint32_t ka[G], kb[G];
+                const uint8_t *row = block + (16 * tile + g) * (D / 2) + 4 * G * t;
+                if (G == 4) {
+                    *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(row);
+                    *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(row + 8 * (D / 2));
+                } else {
+                    *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(row);
+                    *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(row + 8 * (D / 2));
+                }
+                uint32_t da[G / 2], db[G / 2];
+                const uint8_t *scale = block + L::k_scale(16 * tile + g, 0);
+                if (G == 4) {
+                    *reinterpret_cast<uint2 *>(da) = *reinterpret_cast<const uint2 *>(scale);
+                    *reinterpret_cast<uint2 *>(db) = *reinterpret_cast<const uint2 *>(scale + 16 * G);
+                } else {
+                    da[0] = *reinterpret_cast<const uint32_t *>(scale);
+                    db[0] = *reinterpret_cast<const uint32_t *>(scale + 16 * G);
+                }
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    const uint32_t a0[4] = {kv4_low(ka[j]), kv4_low(kb[j]), kv4_high(ka[j]), kv4_high(kb[j])};
+                    const uint32_t a1[4] = {kv4_low(ka[j] >> 8), kv4_low(kb[j] >> 8), kv4_high(ka[j] >> 8),
+                                            kv4_high(kb[j] >> 8)};
+                    const float d0 = j & 1 ? high_half(da[j >> 1]) : low_half(da[j >> 1]);
+                    const float d1 = j & 1 ? high_half(db[j >> 1]) : low_half(db[j >> 1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_16816(c, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+                        mma_16816(c, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+                        acc[nt][0] = fmaf(d0, c[0], acc[nt][0]);
+                        acc[nt][1] = fmaf(d0, c[1], acc[nt][1]);
+                        acc[nt][2] = fmaf(d1, c[2], acc[nt][2]);
+                        acc[nt][3] = fmaf(d1, c[3], acc[nt][3]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const int key = p0 + 16 * tile + g;
+                    sc[tile][nt][0] = key <= limit[nt] ? (acc[nt][0] + acc[nt][1]) * back[nt] : -INFINITY;
+                    sc[tile][nt][1] = key + 8 <= limit[nt] ? (acc[nt][2] + acc[nt][3]) * back[nt] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float mx = m[nt];
+#pragma unroll
+                for (int tile = 0; tile < 4; tile++) mx = fmaxf(mx, fmaxf(sc[tile][nt][0], sc[tile][nt][1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float corr = mx == m[nt] ? 1.0f : exp2f(m[nt] - mx);
+                float sum = 0.0f;
+#pragma unroll
+                for (int tile = 0; tile < 4; tile++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x = sc[tile][nt][e];
+                        sc[tile][nt][e] = x == -INFINITY ? 0.0f : exp2f(x - (mx - kWeightShift));
+                        sum += sc[tile][nt][e];
+                    }
+                l[nt] = fmaf(l[nt], corr, sum);
+                if (__any_sync(0xffffffffu, mx != m[nt])) {
+#pragma unroll
+                    for (int i2 = 0; i2 < MT; i2++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[nt][i2][e] *= corr;
+                }
+                m[nt] = mx;
+            }
+            const int valid = q.length - p0;  // slots behind it hold nothing of this sequence
+            uint32_t poison = 0;              // a NaN scale among the valid ones
+#pragma unroll
+            for (int tile = 0; tile < 4; tile++) {
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x = sc[tile][nt][e];
+                        const __half h = __float2half_rn(x);
+                        const __half2 hl = __halves2half2(h, __float2half_rn(x - __half2float(h)));
+                        pb[nt][e] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&hl));
+                    }
+                uint32_t d2[2];  // scales of keys 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = 16 * tile + 8 * e + 2 * t;
+                    d2[e] = *reinterpret_cast<const uint32_t *>(block + L::v_scale(key, g * (D / 8) / 32));
+                    if (key >= valid) d2[e] = 0;
+                    else if (key + 1 >= valid) d2[e] &= 0xffffu;
+                    // a NaN times a masked row's weight of zero must not reach that row
+                    const uint32_t nan = __hneu2_mask(*reinterpret_cast<__half2 *>(&d2[e]), *reinterpret_cast<__half2 *>(&d2[e]));
+                    poison |= nan;
+                    d2[e] &= ~nan;
+                }
+#pragma unroll
+                for (int w = 0; w < MT / 4; w++) {
+                    uint32_t v[4];  // word w of the lane's dims at keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = *reinterpret_cast<const uint32_t *>(
+                            block + L::v_word(16 * tile + 2 * t + (e & 1) + 8 * (e >> 1), g * (MT / 4) + w));
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const uint32_t x0 = __byte_perm(v[0], v[1], half ? 0x7632 : 0x5410);
+                        const uint32_t x1 = __byte_perm(v[2], v[3], half ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int two = 0; two < 2; two++) {
+                            const uint32_t y0 = two ? x0 >> 8 : x0, y1 = two ? x1 >> 8 : x1;
+                            const uint32_t a[4] = {kv4_times(kv4_low(y0), d2[0]), kv4_times(kv4_high(y0), d2[0]),
+                                                   kv4_times(kv4_low(y1), d2[1]), kv4_times(kv4_high(y1), d2[1])};
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                mma_16816(o[nt][4 * w + 2 * half + two], a, pb[nt][0], pb[nt][1]);
+                        }
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, poison != 0)) {
+                // rare: the rows that see a NaN group get NaN in its dims
+                for (int key = 0; key < min(valid, kPage); key++) {
+                    const float d = __half2float(*reinterpret_cast<const __half *>(block + L::v_scale(key, g * (D / 8) / 32)));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        if (d != d && p0 + key <= limit[nt])
+#pragma unroll
+                            for (int i2 = 0; i2 < MT; i2++) o[nt][i2][0] = o[nt][i2][2] = d;
+                }
+            }
+        }
+        __syncwarp();  // every lane has read the block before it is overwritten
+        if (i + kDecodeStages < mine) issue(i + kDecodeStages, id_of(i + kDecodeStages));
+    }
+    if (!ok) {
+        // copies may be in flight: see them land (bounded) before the CTA's memory goes
+        for (int stage = 0; stage < kDecodeStages; stage++)
+            for (unsigned spin = 0; spin < 1024 && !mbar_test_wait(&bar[stage], phases >> stage & 1); spin++) __nanosleep(500);
+    }
+    __syncthreads();
+    if (*abort_word) {
+        if (threadIdx.x == 0) kv4_report(p.status, kKv4Timeout);
+        return;
+    }
+    // merge the warps' parts, in warp order
+    float *mo = reinterpret_cast<float *>(ring), *ml = mo + kDecodeWarps * K::rows * D;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 4);
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 8);
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 16);
+        const int r = warp * K::rows + 4 * nt + t;
+        float *dst = mo + r * D + g * MT * 2;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+            *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[nt][i][0] + o[nt][i][1], o[nt][i][2] + o[nt][i][3]);
+        if (g == 0) {
+            ml[2 * r] = m[nt];
+            ml[2 * r + 1] = l[nt];
+        }
+    }
+    __syncthreads();
+    constexpr int per = D / 8;  // threads of a row, 8 dims each
+    for (int item = threadIdx.x; item < K::rows * per; item += 32 * kDecodeWarps) {
+        const int r = item / per, d = item % per * 8;
+        if (r0 + r >= n_rows) continue;
+        float top = -INFINITY, total = 0.0f, x[8] = {};
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; w++) top = fmaxf(top, ml[2 * (w * K::rows + r)]);
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; w++) {
+            const int at = w * K::rows + r;
+            // a part without keys has l = 0; one whose scores are NaN has l = NaN and stays
+            const float weight = ml[2 * at + 1] == 0.0f ? 0.0f : ml[2 * at] == top ? 1.0f : exp2f(ml[2 * at] - top);
+            total = fmaf(weight, ml[2 * at + 1], total);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = fmaf(weight, mo[at * D + d + e], x[e]);
+        }
+        if (p.splits == 1) {
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= inverse;
+            const int token = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) - token * p.group;
+            store8(static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + d, p.wide, x);
+        } else {
+            const size_t slot =
+                (((size_t)s * p.cache.heads + kvh) * p.tiles * K::rows + r0 + r) * p.splits + split;
+            float *part = p.part + slot * (D + 2);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(x[e], x[e + 1]);
+            if (d == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(top, total);
+        }
+    }
+}
+
+// One warp per row of a (sequence, KV head): the splits' parts in split order.
+// A block of 4 warps per (sequence, KV head, 4 rows), the rows fastest.
+template <int D, typename T>
+static __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p, int tile_rows)
+{
+    constexpr int per = D / 32;
+    const int lane = threadIdx.x & 31, fours = (tile_rows + 3) / 4, r = blockIdx.x % fours * 4 + (threadIdx.x >> 5);
+    const int kvh = blockIdx.x / fours % p.cache.heads, s = blockIdx.x / fours / p.cache.heads;
+    pdl_wait();
+    pdl_launch_dependents();
+    const Kv4Sequence q = kv4_sequence(p.rows, s);
+    if (!q.ok || r >= q.count * p.group) return;
+    const int pages = (q.length + kPage - 1) / kPage, splits = (pages + p.split_pages - 1) / p.split_pages;
+    const float *part = p.part + (((size_t)s * p.cache.heads + kvh) * tile_rows + r) * p.splits * (D + 2);
+    float top = -INFINITY, total = 0.0f, x[per] = {};
+    for (int i = lane; i < splits; i += 32) top = fmaxf(top, part[(size_t)i * (D + 2) + D]);
+    top = warp_max(top);
+    for (int i0 = 0; i0 < splits; i0 += 32) {
+        float weight = 0.0f;
+        if (i0 + lane < splits) {
+            const float2 ml = *reinterpret_cast<const float2 *>(part + (size_t)(i0 + lane) * (D + 2) + D);
+            weight = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2f(ml.x - top);
+            total = fmaf(weight, ml.y, total);
+        }
+        const int n = min(32, splits - i0);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float w = __shfl_sync(0xffffffffu, weight, i);
+            const float *src = part + (size_t)(i0 + i) * (D + 2) + per * lane;
+#pragma unroll
+            for (int e = 0; e < per; e += 2) {
+                const float2 v = *reinterpret_cast<const float2 *>(src + e);
+                x[e] = fmaf(w, v.x, x[e]);
+                x[e + 1] = fmaf(w, v.y, x[e + 1]);
             }
         }
     }
-    T *dst = static_cast<T *>(p.out) + (size_t)row * p.out_stride + (size_t)head * D + lane * per;
-    for (int e = 0; e < per; e++) dst[e] = from_float<T>(l == 0.0f ? 0.0f : o[e] / l);
+    total = warp_sum(total);
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const int token = r / p.group, head = kvh * p.group + r - token * p.group;
+    T *dst = static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + per * lane;
+#pragma unroll
+    for (int e = 0; e < per; e++) dst[e] = from_float<T>(x[e] * inverse);
 }
 
 }  // namespace lun

@@ -98,10 +98,10 @@ def query_scale(position):
 def attention(q, k, v, scale, first_position):
     """Rows q [n, query heads, dim] at first_position.. over k, v [length, heads, dim]. Returns the
     output and, for error bounds, per row and head the largest sum |q_d k_d| * |scale| over visible
-    keys and sum p |v| per dim."""
+    keys, and sum p |v| and sum |v| per dim."""
     n, qh, dim = q.shape
     group = qh // k.shape[1]
-    out, spread, weight = np.zeros((n, qh, dim)), np.zeros((n, qh)), np.zeros((n, qh, dim))
+    out, spread, weight, total = np.zeros((n, qh, dim)), np.zeros((n, qh)), np.zeros((n, qh, dim)), np.zeros((n, qh, dim))
     for i in range(n):
         seen = min(first_position + i + 1, k.shape[0])
         if seen <= 0:
@@ -114,4 +114,5 @@ def attention(q, k, v, scale, first_position):
             out[i, h] = p @ vv
             spread[i, h] = abs(scale) * (np.abs(kk) @ np.abs(q[i, h])).max()
             weight[i, h] = p @ np.abs(vv)
-    return out, spread, weight
+            total[i, h] = np.abs(vv).sum(0)
+    return out, spread, weight, total
