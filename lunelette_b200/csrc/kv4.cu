@@ -180,18 +180,24 @@ struct AttnPlan {
     size_t part_bytes;
 };
 
-static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows, size_t query_heads)
+static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows, size_t query_heads,
+                               int type)
 {
     AttnPlan a;
     const size_t group = query_heads / cache->kv_heads, most = rows->max_count * group;
-    a.nt = most <= 4 ? 1 : 2;
-    a.tile_rows = 4 * a.nt;
+    const int lane = type == LUNELETTE_CUDA_FLOAT32 ? 4 : 8;  // rows of an n tile
+    a.nt = most <= (size_t)lane ? 1 : 2;
+    a.tile_rows = lane * a.nt;
     a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
     const size_t pages = (rows->max_length + kPage - 1) / kPage;
-    const size_t items = rows->sequences * cache->kv_heads * a.tiles;
-    size_t per = pages * items / (2 * 148);
-    per = per < 4 ? 4 : per > 64 ? 64 : per;
-    a.split_pages = (int)((per + 3) / 4 * 4);
+    const size_t items = rows->sequences * cache->kv_heads * a.tiles, slots = 148 * (a.nt == 1 ? kDecodeCtas : 2);
+    // one wave of CTAs where that leaves each warp a page or more; where there
+    // are more items than CTAs, parts of 16 pages, so that long sequences do not
+    // outlast the short ones
+    size_t splits = slots / (items ? items : 1), per = splits ? (pages + splits - 1) / splits : 16;
+    if (per > 16 && items * 4 > slots) per = 16;
+    a.split_pages = (int)((per + kDecodeWarps - 1) / kDecodeWarps * kDecodeWarps);
+    if (a.split_pages < kDecodeWarps) a.split_pages = kDecodeWarps;
     a.splits = (int)((pages + a.split_pages - 1) / a.split_pages);
     if (a.splits < 1) a.splits = 1;
     a.part_bytes = a.splits == 1 ? 0 : items * a.tile_rows * a.splits * (cache->head_dim + 2) * sizeof(float);
@@ -205,20 +211,22 @@ LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *
     if (!valid_cache(cache, 0) || !valid_rows(rows, &empty) || !query_heads || query_heads > 4096 ||
         query_heads % cache->kv_heads || empty)
         return 0;
-    return plan_attention(cache, rows, query_heads).part_bytes;
+    const size_t wide = plan_attention(cache, rows, query_heads, LUNELETTE_CUDA_FLOAT32).part_bytes;
+    const size_t narrow = plan_attention(cache, rows, query_heads, LUNELETTE_CUDA_FLOAT16).part_bytes;
+    return wide > narrow ? wide : narrow;
 }
 
 template <int D, typename T, int NT>
 static cudaError_t launch_decode(const Kv4AttnParams &p, const AttnPlan &a, int sequences, cudaStream_t stream)
 {
-    constexpr int smem = Kv4Decode<D, NT>::smem;
+    constexpr int smem = Kv4Decode<D, T, NT>::smem;
     auto kernel = kv4_decode_kernel<D, T, NT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const size_t items = (size_t)sequences * p.cache.heads * a.tiles;
     e = launch(kernel, dim3((unsigned)(items * a.splits)), dim3(32 * kDecodeWarps), smem, stream, p);
     if (e != cudaSuccess || a.splits == 1) return e;
-    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * a.nt)), dim3(128), 0, stream, p, a.tiles * a.tile_rows);
+    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * ((a.tile_rows + 3) / 4))), dim3(128), 0, stream, p, a.tiles * a.tile_rows);
 }
 
 LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer,
@@ -234,7 +242,7 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
         !valid_tensor(out, out_stride, width, type, empty, &wide) || !aligned(status, 4) || !aligned(workspace, 16))
         return -1;
     if (empty) return 0;
-    const AttnPlan a = plan_attention(cache, rows, query_heads);
+    const AttnPlan a = plan_attention(cache, rows, query_heads, type);
     if (workspace_bytes < a.part_bytes || (a.part_bytes && !workspace)) return -1;
     if (rows->sequences * cache->kv_heads * a.tiles > (size_t)INT_MAX / a.splits) return -1;
     Kv4AttnParams p;

@@ -1,18 +1,21 @@
 // Causal attention over the paged 4-bit KV cache for few query rows: decode
 // steps over many sequences, and short runs of tokens.
 //
-// HBM-bound by design: a block of the cache (one page of one KV head, K and V with their
-// scales, 9216 bytes for 128 dims) is copied once into shared memory by one bulk
-// copy and serves all the query rows of its KV head. Each warp walks pages of its
-// own with its own ring of blocks, so nothing waits for another warp until the
-// last merge; keys split over warps, CTAs (splits) and, in the combine kernel,
-// back together in a fixed order.
+// HBM-bound by design: a block of the cache (one page of one KV head, 9216 bytes for
+// 128 dims) is copied once into shared memory, K with its scales and V with its
+// scales by one bulk copy each, and serves all the query rows of its KV head. Each
+// warp walks pages of its own with its own ring of half blocks, so nothing waits for
+// another warp until the last merge; keys split over warps, CTAs (splits) and, in
+// the combine kernel, back together in a fixed order.
 //
 // The products run on mma.sync m16n8k16 with FP16 operands and FP32 sums: a
-// decode step has 1 to 8 query rows a KV head, so a tcgen05 tile of 128 rows would be
-// 94% padding, while here the rows sit in the n = 8 side. FP32 rows of q and
+// decode step has 1 to 16 query rows a KV head, so a tcgen05 tile of 128 rows would be
+// mostly padding, while here the rows sit in the n = 8 side. FP32 rows of q and
 // weights of the softmax enter as FP16 hi + lo parts in neighbouring columns
-// (22 bits together), so one MMA serves 4 rows at FP32 grade.
+// (22 bits together), so one MMA serves 4 rows at FP32 grade; of 16-bit rows the 11
+// bits of one FP16 are taken (q exact after a power-of-two scaling but for what lies
+// 2^-17 below the row's largest; a weight off by 2^-12 of itself, under the rounding of the
+// output), 8 rows an MMA.
 //   S = K Q^T     A: 16 keys x 16 dims of integers c - 8 straight from the
 //                 codes (exact); a group's sum is scaled by d in FP32 after its
 //                 two MMAs, so K needs no multiplication per element.
@@ -53,14 +56,30 @@ static __device__ int kv4_error_sink;
 // subnormals.
 constexpr float kWeightShift = 14.0f;
 
-constexpr int kDecodeWarps = 4, kDecodeStages = 3;
+#ifndef KV4_WARPS
+#define KV4_WARPS 4
+#define KV4_SLOTS 3
+#define KV4_CTAS 4
+#endif
+constexpr int kDecodeWarps = KV4_WARPS, kDecodeSlots = KV4_SLOTS, kDecodeCtas = KV4_CTAS;
 
-template <int D, int NT> struct Kv4Decode {
-    static constexpr int rows = 4 * NT;  // query rows of a tile
-    static constexpr int ring = kDecodeWarps * kDecodeStages * Kv4Layout<D>::block;
+template <int D, typename T, int NT> struct Kv4Decode {
+    static constexpr bool split = sizeof(T) == 4;    // hi and lo columns
+    static constexpr int lane_rows = split ? 1 : 2;  // query rows of a lane and n tile
+    static constexpr int rows = 4 * NT * lane_rows;  // query rows of a tile
+    static constexpr int half = Kv4Layout<D>::block / 2;
+    static constexpr int ring = kDecodeWarps * kDecodeSlots * half;
     static constexpr int merge = kDecodeWarps * rows * (D + 2) * 4;
-    static constexpr int smem = 128 + (ring > merge ? ring : merge) + kDecodeWarps * kDecodeStages * 8 + 16;
+    static constexpr int bars = (ring > merge ? ring : merge);
+    static constexpr int smem = bars + kDecodeWarps * kDecodeSlots * 8 + 16;
 };
+
+__device__ __forceinline__ float exp2_fast(float x)  // 2 ulp; 0 below 2^-126
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 // Four codes in the bytes' low and high nibbles of both halves -> c - 8 in FP16:
 // a = (nibble 0, nibble 4), b = (nibble 1, nibble 5) of a word.
@@ -107,18 +126,22 @@ __device__ __forceinline__ float power_scale(float x, float &back)
 
 // A block per (sequence, KV head, row tile, split), the split fastest.
 template <int D, typename T, int NT>
-static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv4AttnParams p)
+static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCtas : 2) kv4_decode_kernel(Kv4AttnParams p)
 {
     using L = Kv4Layout<D>;
-    using K = Kv4Decode<D, NT>;
-    constexpr int G = L::groups, MT = D / 16;  // m tiles of V's dims
+    using K = Kv4Decode<D, T, NT>;
+    constexpr int G = L::groups, MT = D / 16, RP = K::lane_rows, W = kDecodeWarps, SLOTS = kDecodeSlots;
+    constexpr int row_bytes = D / 2;
     extern __shared__ __align__(128) uint8_t kv4_smem[];
-    uint8_t *ring = kv4_smem;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(kv4_smem + K::smem - kDecodeWarps * kDecodeStages * 8 - 16);
-    volatile int *abort_word = reinterpret_cast<volatile int *>(bars + kDecodeWarps * kDecodeStages);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(kv4_smem + K::bars);
+    volatile int *abort_word = reinterpret_cast<volatile int *>(bars + W * SLOTS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % p.splits, tile_of = blockIdx.x / p.splits, r0 = tile_of % p.tiles * K::rows;
     const int kvh = tile_of / p.tiles % p.cache.heads, s = tile_of / p.tiles / p.cache.heads;
+    uint64_t *bar = bars + warp * SLOTS;
+    if (threadIdx.x == 0) *abort_word = 0;
+    if (lane < SLOTS) mbar_init(&bar[lane], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pdl_wait();
     pdl_launch_dependents();
     const Kv4Sequence q = kv4_sequence(p.rows, s);
@@ -130,35 +153,34 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv
     if (r0 >= n_rows) return;
     const int pages = (q.length + kPage - 1) / kPage, first = split * p.split_pages;
     const int last = min(first + p.split_pages, pages);  // this split's pages [first, last)
-    if (first >= last && (split > 0 || p.splits > 1)) return;  // the combine knows how many splits have pages
-    if (threadIdx.x == 0) *abort_word = 0;
-    if (lane < kDecodeStages) mbar_init(&bars[warp * kDecodeStages + lane], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (first >= last && p.splits > 1) return;           // the combine knows how many splits have pages
     __syncthreads();
 
-    // the warp's pages are first + warp + 4 i; their ids, 32 at a time, one a lane
+    // the warp's pages are first + warp + W i; their ids, 32 at a time, one a lane
     const int *table = p.rows.page_tables + s * p.rows.table_stride;
-    const int mine = last - first - warp > 0 ? (last - first - warp + kDecodeWarps - 1) / kDecodeWarps : 0;
-    uint8_t *buffers = ring + warp * kDecodeStages * L::block;
-    uint64_t *bar = bars + warp * kDecodeStages;
-    int ids = lane < mine ? table[first + warp + lane * kDecodeWarps] : 0;
+    const int mine = last - first - warp > 0 ? (last - first - warp + W - 1) / W : 0;
+    uint8_t *buffers = kv4_smem + warp * SLOTS * K::half;
+    int ids = lane < mine ? table[first + warp + lane * W] : 0;
     int next_ids = 0;
     auto id_of = [&](int i) { return __shfl_sync(0xffffffffu, (i & 32) ? next_ids : ids, i & 31); };
-    auto issue = [&](int i, int id) {
-        const uint8_t *block = kv4_block<D>(p.cache, id, kvh);
+    // half h of the walk: K (even) or V (odd) of the warp's page h / 2
+    auto issue = [&](int h, int slot) {
+        const uint8_t *block = kv4_block<D>(p.cache, id_of(h >> 1), kvh);
         if (lane == 0 && block) {
-            mbar_expect_tx(&bar[i % kDecodeStages], L::block);
-            bulk_g2s(buffers + i % kDecodeStages * L::block, block, L::block, &bar[i % kDecodeStages]);
+            mbar_expect_tx(&bar[slot], K::half);
+            bulk_g2s(buffers + slot * K::half, block + (h & 1 ? K::half : 0), K::half, &bar[slot]);
         }
     };
-    // q: two columns (hi, lo) a row; column g belongs to row g / 2
+#pragma unroll
+    for (int h = 0; h < SLOTS; h++)
+        if (h < 2 * mine) issue(h, h);
+    // q as B: column g of n tile nt belongs to row (split: 4 nt + g / 2, part g % 2; else 8 nt + g)
     uint32_t qb[NT][D / 16][2];
-    float back[NT];  // what a score is multiplied with, of row nt * 4 + t
-    int limit[NT];   // that row's last visible position
-    for (int i = 0; i < kDecodeStages && i < mine; i++) issue(i, id_of(i));
+    float back[NT][RP];  // what a score is multiplied with, of the lane's rows 4 nt + t or 8 nt + 2 t + (0, 1)
+    int limit[NT][RP];   // those rows' last visible position
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = r0 + 4 * nt + (g >> 1);
+        const int r = r0 + (K::split ? 4 * nt + (g >> 1) : 8 * nt + g);
         const bool live = r < n_rows;
         const int token = live ? r / p.group : 0, head = kvh * p.group + (live ? r - token * p.group : 0);
         const T *src = static_cast<const T *>(p.q) + (size_t)(q.first + token) * p.q_stride + (size_t)head * D + 8 * t;
@@ -176,8 +198,6 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         float undo;
         const float f = power_scale(top, undo);
-        // lane (g, t) scores row 4 nt + t, whose factors sit in lane (2 t, .)
-        back[nt] = __shfl_sync(0xffffffffu, undo, 8 * t) * p.scale2;
 #pragma unroll
         for (int j = 0; j < G; j++)
 #pragma unroll
@@ -186,181 +206,241 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv
                 for (int b = 0; b < 2; b++) {
                     uint32_t hi, lo;
                     split_half2(x[j][2 * hw + b] * f, x[j][2 * hw + b + 4] * f, hi, lo);
-                    qb[nt][2 * j + hw][b] = g & 1 ? lo : hi;
+                    qb[nt][2 * j + hw][b] = K::split && (g & 1) ? lo : hi;
                 }
-        const int mine_r = r0 + 4 * nt + t;
-        limit[nt] = mine_r < n_rows ? q.length - q.count + mine_r / p.group : -1;
+#pragma unroll
+        for (int e = 0; e < RP; e++) {
+            // the row's factors sit in the lanes of its (first) column
+            back[nt][e] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + e)) * p.scale2;
+            const int row = r0 + (K::split ? 4 * nt + t : 8 * nt + 2 * t + e);
+            limit[nt][e] = row < n_rows ? q.length - q.count + row / p.group : -1;
+        }
     }
-    float m[NT], l[NT], o[NT][MT][4];
+    const int all_see = q.length - q.count + r0 / p.group;  // every row of the tile sees keys up to here
+    float m[NT][RP], l[NT][RP], o[NT][MT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        m[nt] = -INFINITY;
-        l[nt] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < RP; e++) {
+            m[nt][e] = -INFINITY;
+            l[nt][e] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < MT; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
     }
+    // byte offsets of the lane's first reads in a half block; 16 keys on are 16 rows on, the swizzle the same
+    const int k_at = g * row_bytes + 4 * G * t, ks_at = L::k_scale(g, 0);
+    const int v_even = L::v_word(2 * t, g * (MT / 4)) - K::half, v_odd = v_even ^ row_bytes;
+    const int vs_at = L::v_scale(2 * t, g * (D / 8) / 32) - K::half;
     bool ok = true;
-    unsigned phases = 0;  // parity of each stage's next wait
+    unsigned phases = 0;  // parity of each slot's next wait
+    int slot = 0;
+    auto next = [&](int h) {  // done with half h: every lane has read it; refill its slot
+        __syncwarp();
+        if (h + SLOTS < 2 * mine) issue(h + SLOTS, slot);
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+    };
     for (int i = 0; i < mine; i++) {
         if ((i & 31) == 0 && i + 32 < mine) {  // the other half of the ids, long before it is asked for
-            const int fetched = i + 32 + lane < mine ? table[first + warp + (i + 32 + lane) * kDecodeWarps] : 0;
+            const int fetched = i + 32 + lane < mine ? table[first + warp + (i + 32 + lane) * W] : 0;
             if (i & 32) ids = fetched;
             else next_ids = fetched;
         }
-        const int stage = i % kDecodeStages, page_index = first + warp + i * kDecodeWarps;
-        const int id = id_of(i);
-        if ((unsigned)id >= (unsigned)p.cache.pages) {
+        if ((unsigned)id_of(i) >= (unsigned)p.cache.pages) {
             if (lane == 0) kv4_report(p.status, kKv4BadPage);
-        } else {
-            ok = warp_wait(&bar[stage], phases >> stage & 1, abort_word, &kv4_error_sink);
-            if (!ok) break;
-            phases ^= 1u << stage;
-            const uint8_t *block = buffers + stage * L::block;
-            const int p0 = page_index * kPage;
-            float sc[4][NT][2];
+            next(2 * i);
+            next(2 * i + 1);
+            continue;
+        }
+        if (!(ok = warp_wait(&bar[slot], phases >> slot & 1, abort_word, &kv4_error_sink))) break;
+        phases ^= 1u << slot;
+        const uint8_t *block = buffers + slot * K::half;
+        const int p0 = (first + warp + i * W) * kPage;
+        float sc[4][NT][2][RP];
 #pragma unroll
-            for (int tile = 0; tile < 4; tile++) {
-                float acc[NT][4];
+        for (int tile = 0; tile < 4; tile++) {
+            float acc[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
-                uint32_t ka[G], kb[G];
-                const uint8_t *row = block + (16 * tile + g) * (D / 2) + 4 * G * t;
-                if (G == 4) {
-                    *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(row);
-                    *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(row + 8 * (D / 2));
-                } else {
-                    *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(row);
-                    *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(row + 8 * (D / 2));
-                }
-                uint32_t da[G / 2], db[G / 2];
-                const uint8_t *scale = block + L::k_scale(16 * tile + g, 0);
-                if (G == 4) {
-                    *reinterpret_cast<uint2 *>(da) = *reinterpret_cast<const uint2 *>(scale);
-                    *reinterpret_cast<uint2 *>(db) = *reinterpret_cast<const uint2 *>(scale + 16 * G);
-                } else {
-                    da[0] = *reinterpret_cast<const uint32_t *>(scale);
-                    db[0] = *reinterpret_cast<const uint32_t *>(scale + 16 * G);
-                }
+            for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+            uint32_t ka[G], kb[G], da[G / 2], db[G / 2];
+            const uint8_t *row = block + k_at + 16 * tile * row_bytes, *scale = block + ks_at + 32 * G * tile;
+            if constexpr (G == 4) {
+                *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(row);
+                *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(row + 8 * row_bytes);
+                *reinterpret_cast<uint2 *>(da) = *reinterpret_cast<const uint2 *>(scale);
+                *reinterpret_cast<uint2 *>(db) = *reinterpret_cast<const uint2 *>(scale + 16 * G);
+            } else {
+                *reinterpret_cast<uint2 *>(ka) = *reinterpret_cast<const uint2 *>(row);
+                *reinterpret_cast<uint2 *>(kb) = *reinterpret_cast<const uint2 *>(row + 8 * row_bytes);
+                da[0] = *reinterpret_cast<const uint32_t *>(scale);
+                db[0] = *reinterpret_cast<const uint32_t *>(scale + 16 * G);
+            }
 #pragma unroll
-                for (int j = 0; j < G; j++) {
-                    const uint32_t a0[4] = {kv4_low(ka[j]), kv4_low(kb[j]), kv4_high(ka[j]), kv4_high(kb[j])};
-                    const uint32_t a1[4] = {kv4_low(ka[j] >> 8), kv4_low(kb[j] >> 8), kv4_high(ka[j] >> 8),
-                                            kv4_high(kb[j] >> 8)};
-                    const float d0 = j & 1 ? high_half(da[j >> 1]) : low_half(da[j >> 1]);
-                    const float d1 = j & 1 ? high_half(db[j >> 1]) : low_half(db[j >> 1]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_16816(c, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
-                        mma_16816(c, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
-                        acc[nt][0] = fmaf(d0, c[0], acc[nt][0]);
-                        acc[nt][1] = fmaf(d0, c[1], acc[nt][1]);
-                        acc[nt][2] = fmaf(d1, c[2], acc[nt][2]);
-                        acc[nt][3] = fmaf(d1, c[3], acc[nt][3]);
-                    }
-                }
+            for (int j = 0; j < G; j++) {
+                const uint32_t a0[4] = {kv4_low(ka[j]), kv4_low(kb[j]), kv4_high(ka[j]), kv4_high(kb[j])};
+                const uint32_t a1[4] = {kv4_low(ka[j] >> 8), kv4_low(kb[j] >> 8), kv4_high(ka[j] >> 8),
+                                        kv4_high(kb[j] >> 8)};
+                const float d0 = j & 1 ? high_half(da[j >> 1]) : low_half(da[j >> 1]);
+                const float d1 = j & 1 ? high_half(db[j >> 1]) : low_half(db[j >> 1]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const int key = p0 + 16 * tile + g;
-                    sc[tile][nt][0] = key <= limit[nt] ? (acc[nt][0] + acc[nt][1]) * back[nt] : -INFINITY;
-                    sc[tile][nt][1] = key + 8 <= limit[nt] ? (acc[nt][2] + acc[nt][3]) * back[nt] : -INFINITY;
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_16816(c, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+                    mma_16816(c, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+                    acc[nt][0] = fmaf(d0, c[0], acc[nt][0]);
+                    acc[nt][1] = fmaf(d0, c[1], acc[nt][1]);
+                    acc[nt][2] = fmaf(d1, c[2], acc[nt][2]);
+                    acc[nt][3] = fmaf(d1, c[3], acc[nt][3]);
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float mx = m[nt];
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int tile = 0; tile < 4; tile++) mx = fmaxf(mx, fmaxf(sc[tile][nt][0], sc[tile][nt][1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float corr = mx == m[nt] ? 1.0f : exp2f(m[nt] - mx);
-                float sum = 0.0f;
-#pragma unroll
-                for (int tile = 0; tile < 4; tile++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float x = sc[tile][nt][e];
-                        sc[tile][nt][e] = x == -INFINITY ? 0.0f : exp2f(x - (mx - kWeightShift));
-                        sum += sc[tile][nt][e];
+                for (int k8 = 0; k8 < 2; k8++) {
+                    if constexpr (K::split) {
+                        sc[tile][nt][k8][0] = (acc[nt][2 * k8] + acc[nt][2 * k8 + 1]) * back[nt][0];
+                    } else {
+                        sc[tile][nt][k8][0] = acc[nt][2 * k8] * back[nt][0];
+                        sc[tile][nt][k8][1] = acc[nt][2 * k8 + 1] * back[nt][1];
                     }
-                l[nt] = fmaf(l[nt], corr, sum);
-                if (__any_sync(0xffffffffu, mx != m[nt])) {
-#pragma unroll
-                    for (int i2 = 0; i2 < MT; i2++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[nt][i2][e] *= corr;
                 }
-                m[nt] = mx;
-            }
-            const int valid = q.length - p0;  // slots behind it hold nothing of this sequence
-            uint32_t poison = 0;              // a NaN scale among the valid ones
+        }
+        next(2 * i);
+        if (p0 + kPage - 1 > all_see) {
 #pragma unroll
-            for (int tile = 0; tile < 4; tile++) {
-                uint32_t pb[NT][2];
+            for (int tile = 0; tile < 4; tile++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float x = sc[tile][nt][e];
-                        const __half h = __float2half_rn(x);
-                        const __half2 hl = __halves2half2(h, __float2half_rn(x - __half2float(h)));
-                        pb[nt][e] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&hl));
-                    }
-                uint32_t d2[2];  // scales of keys 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
+                    for (int k8 = 0; k8 < 2; k8++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = 16 * tile + 8 * e + 2 * t;
-                    d2[e] = *reinterpret_cast<const uint32_t *>(block + L::v_scale(key, g * (D / 8) / 32));
-                    if (key >= valid) d2[e] = 0;
-                    else if (key + 1 >= valid) d2[e] &= 0xffffu;
-                    // a NaN times a masked row's weight of zero must not reach that row
-                    const uint32_t nan = __hneu2_mask(*reinterpret_cast<__half2 *>(&d2[e]), *reinterpret_cast<__half2 *>(&d2[e]));
-                    poison |= nan;
-                    d2[e] &= ~nan;
-                }
+                        for (int e = 0; e < RP; e++)
+                            if (p0 + 16 * tile + 8 * k8 + g > limit[nt][e]) sc[tile][nt][k8][e] = -INFINITY;
+        }
+        uint32_t pb[4][NT][2];
 #pragma unroll
-                for (int w = 0; w < MT / 4; w++) {
-                    uint32_t v[4];  // word w of the lane's dims at keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        for (int nt = 0; nt < NT; nt++) {
+            float corr[RP], base[RP];
+            bool raised = false;
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        v[e] = *reinterpret_cast<const uint32_t *>(
-                            block + L::v_word(16 * tile + 2 * t + (e & 1) + 8 * (e >> 1), g * (MT / 4) + w));
+            for (int e = 0; e < RP; e++) {
+                float mx = m[nt][e];
 #pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        const uint32_t x0 = __byte_perm(v[0], v[1], half ? 0x7632 : 0x5410);
-                        const uint32_t x1 = __byte_perm(v[2], v[3], half ? 0x7632 : 0x5410);
-#pragma unroll
-                        for (int two = 0; two < 2; two++) {
-                            const uint32_t y0 = two ? x0 >> 8 : x0, y1 = two ? x1 >> 8 : x1;
-                            const uint32_t a[4] = {kv4_times(kv4_low(y0), d2[0]), kv4_times(kv4_high(y0), d2[0]),
-                                                   kv4_times(kv4_low(y1), d2[1]), kv4_times(kv4_high(y1), d2[1])};
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-                                mma_16816(o[nt][4 * w + 2 * half + two], a, pb[nt][0], pb[nt][1]);
-                        }
-                    }
-                }
+                for (int tile = 0; tile < 4; tile++) mx = fmaxf(mx, fmaxf(sc[tile][nt][0][e], sc[tile][nt][1][e]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                raised = raised || mx != m[nt][e];
+                corr[e] = mx == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - mx);
+                m[nt][e] = mx;
+                // a row without any key yet: exp2(-inf - 0) = 0
+                base[e] = mx == -INFINITY ? 0.0f : mx - kWeightShift;
+                l[nt][e] *= corr[e];
             }
-            if (__any_sync(0xffffffffu, poison != 0)) {
-                // rare: the rows that see a NaN group get NaN in its dims
-                for (int key = 0; key < min(valid, kPage); key++) {
-                    const float d = __half2float(*reinterpret_cast<const __half *>(block + L::v_scale(key, g * (D / 8) / 32)));
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        if (d != d && p0 + key <= limit[nt])
+            for (int tile = 0; tile < 4; tile++)
 #pragma unroll
-                            for (int i2 = 0; i2 < MT; i2++) o[nt][i2][0] = o[nt][i2][2] = d;
+                for (int k8 = 0; k8 < 2; k8++) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < RP; e++) {
+                        w[e] = exp2_fast(sc[tile][nt][k8][e] - base[e]);
+                        l[nt][e] += w[e];
+                    }
+                    __half2 two;
+                    if constexpr (K::split) {
+                        const __half h = __float2half_rn(w[0]);
+                        two = __halves2half2(h, __float2half_rn(w[0] - __half2float(h)));
+                    } else {
+                        two = __floats2half2_rn(w[0], w[1]);
+                    }
+                    pb[tile][nt][k8] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&two));
                 }
+            if (__any_sync(0xffffffffu, raised)) {
+#pragma unroll
+                for (int i2 = 0; i2 < MT; i2++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[nt][i2][e] *= corr[K::split ? 0 : e & 1];
             }
         }
-        __syncwarp();  // every lane has read the block before it is overwritten
-        if (i + kDecodeStages < mine) issue(i + kDecodeStages, id_of(i + kDecodeStages));
+        if (!(ok = warp_wait(&bar[slot], phases >> slot & 1, abort_word, &kv4_error_sink))) break;
+        phases ^= 1u << slot;
+        uint8_t *vblock = buffers + slot * K::half;
+        {
+            // scales behind the last position (whatever those slots hold) and NaNs become zeros
+            // before the MMAs, in which a weight of zero would not keep a NaN away from a row
+            // that does not see its position; the rows that do see a NaN take it here
+            constexpr int own = kPage * G / 32;  // scales of a lane, [position / 2][group][position % 2]
+            uint8_t *mine_at = vblock + L::v_scale(0, 0) - K::half + 2 * own * lane;
+            uint32_t d[own / 2];
+            if constexpr (own == 8) *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(mine_at);
+            else *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(mine_at);
+            const int valid = q.length - p0;
+            uint32_t nan = 0;
+#pragma unroll
+            for (int e = 0; e < own / 2; e++) nan |= __hneu2_mask(*reinterpret_cast<__half2 *>(&d[e]), *reinterpret_cast<__half2 *>(&d[e]));
+            if (valid < kPage || __any_sync(0xffffffffu, nan != 0)) {
+                for (int key = 0; key < min(valid, kPage); key++) {
+                    const float x = __half2float(*reinterpret_cast<const __half *>(vblock + L::v_scale(key, g * (D / 8) / 32) - K::half));
+                    if (x != x)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < RP; e++)
+                                if (p0 + key <= limit[nt][e])
+#pragma unroll
+                                    for (int i2 = 0; i2 < MT; i2++) o[nt][i2][e] = o[nt][i2][2 + e] = x;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < own / 2; e++) {
+                    d[e] &= ~__hneu2_mask(*reinterpret_cast<__half2 *>(&d[e]), *reinterpret_cast<__half2 *>(&d[e]));
+                    const int key = (own * lane / (2 * G) + e / G) * 2;
+                    if (key >= valid) d[e] = 0;
+                    else if (key + 1 >= valid) d[e] &= 0xffffu;
+                    reinterpret_cast<uint32_t *>(mine_at)[e] = d[e];
+                }
+                fence_proxy_async_smem();  // before the slot's next bulk copy
+                __syncwarp();
+            }
+        }
+#pragma unroll
+        for (int tile = 0; tile < 4; tile++) {
+            uint32_t d2[2], v[4][MT / 4];
+            const uint8_t *rows16 = vblock + 16 * tile * row_bytes;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                d2[e] = *reinterpret_cast<const uint32_t *>(vblock + vs_at + (16 * tile + 8 * e) * 2 * G);
+#pragma unroll
+                for (int odd = 0; odd < 2; odd++) {
+                    const uint8_t *at = rows16 + (odd ? v_odd : v_even) + 8 * e * row_bytes;
+                    if constexpr (MT == 8) *reinterpret_cast<uint2 *>(v[2 * e + odd]) = *reinterpret_cast<const uint2 *>(at);
+                    else v[2 * e + odd][0] = *reinterpret_cast<const uint32_t *>(at);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < MT / 4; w++)
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const uint32_t x0 = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+                    const uint32_t x1 = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (int two = 0; two < 2; two++) {
+                        const uint32_t y0 = two ? x0 >> 8 : x0, y1 = two ? x1 >> 8 : x1;
+                        const uint32_t a[4] = {kv4_times(kv4_low(y0), d2[0]), kv4_times(kv4_high(y0), d2[0]),
+                                               kv4_times(kv4_low(y1), d2[1]), kv4_times(kv4_high(y1), d2[1])};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            mma_16816(o[nt][4 * w + 2 * half + two], a, pb[tile][nt][0], pb[tile][nt][1]);
+                    }
+                }
+        }
+        next(2 * i + 1);
     }
     if (!ok) {
         // copies may be in flight: see them land (bounded) before the CTA's memory goes
-        for (int stage = 0; stage < kDecodeStages; stage++)
-            for (unsigned spin = 0; spin < 1024 && !mbar_test_wait(&bar[stage], phases >> stage & 1); spin++) __nanosleep(500);
+        for (int i = 0; i < SLOTS; i++)
+            for (unsigned spin = 0; spin < 1024 && !mbar_test_wait(&bar[i], phases >> i & 1); spin++) __nanosleep(500);
     }
     __syncthreads();
     if (*abort_word) {
@@ -368,35 +448,40 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv
         return;
     }
     // merge the warps' parts, in warp order
-    float *mo = reinterpret_cast<float *>(ring), *ml = mo + kDecodeWarps * K::rows * D;
+    float *mo = reinterpret_cast<float *>(kv4_smem), *ml = mo + W * K::rows * D;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 4);
-        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 8);
-        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], 16);
-        const int r = warp * K::rows + 4 * nt + t;
-        float *dst = mo + r * D + g * MT * 2;
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int i = 0; i < MT; i++)
-            *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[nt][i][0] + o[nt][i][1], o[nt][i][2] + o[nt][i][3]);
-        if (g == 0) {
-            ml[2 * r] = m[nt];
-            ml[2 * r + 1] = l[nt];
+        for (int e = 0; e < RP; e++) {
+            float sum = l[nt][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int r = warp * K::rows + (K::split ? 4 * nt + t : 8 * nt + 2 * t + e);
+            float *dst = mo + r * D + g * MT * 2;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+                *reinterpret_cast<float2 *>(dst + 2 * i) =
+                    K::split ? make_float2(o[nt][i][0] + o[nt][i][1], o[nt][i][2] + o[nt][i][3])
+                             : make_float2(o[nt][i][e], o[nt][i][2 + e]);
+            if (g == 0) {
+                ml[2 * r] = m[nt][e];
+                ml[2 * r + 1] = sum;
+            }
         }
-    }
     __syncthreads();
     constexpr int per = D / 8;  // threads of a row, 8 dims each
-    for (int item = threadIdx.x; item < K::rows * per; item += 32 * kDecodeWarps) {
+    for (int item = threadIdx.x; item < K::rows * per; item += 32 * W) {
         const int r = item / per, d = item % per * 8;
         if (r0 + r >= n_rows) continue;
         float top = -INFINITY, total = 0.0f, x[8] = {};
 #pragma unroll
-        for (int w = 0; w < kDecodeWarps; w++) top = fmaxf(top, ml[2 * (w * K::rows + r)]);
+        for (int w = 0; w < W; w++) top = fmaxf(top, ml[2 * (w * K::rows + r)]);
 #pragma unroll
-        for (int w = 0; w < kDecodeWarps; w++) {
+        for (int w = 0; w < W; w++) {
             const int at = w * K::rows + r;
             // a part without keys has l = 0; one whose scores are NaN has l = NaN and stays
-            const float weight = ml[2 * at + 1] == 0.0f ? 0.0f : ml[2 * at] == top ? 1.0f : exp2f(ml[2 * at] - top);
+            const float weight = ml[2 * at + 1] == 0.0f ? 0.0f : ml[2 * at] == top ? 1.0f : exp2_fast(ml[2 * at] - top);
             total = fmaf(weight, ml[2 * at + 1], total);
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = fmaf(weight, mo[at * D + d + e], x[e]);
@@ -408,9 +493,9 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps) kv4_decode_kernel(Kv
             const int token = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) - token * p.group;
             store8(static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + d, p.wide, x);
         } else {
-            const size_t slot =
+            const size_t slot_of =
                 (((size_t)s * p.cache.heads + kvh) * p.tiles * K::rows + r0 + r) * p.splits + split;
-            float *part = p.part + slot * (D + 2);
+            float *part = p.part + slot_of * (D + 2);
 #pragma unroll
             for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(x[e], x[e + 1]);
             if (d == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(top, total);
@@ -439,7 +524,7 @@ static __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p
         float weight = 0.0f;
         if (i0 + lane < splits) {
             const float2 ml = *reinterpret_cast<const float2 *>(part + (size_t)(i0 + lane) * (D + 2) + D);
-            weight = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2f(ml.x - top);
+            weight = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2_fast(ml.x - top);
             total = fmaf(weight, ml.y, total);
         }
         const int n = min(32, splits - i0);
