@@ -1,5 +1,5 @@
 // C-ABI of the 4-bit KV cache (include/lunelette_cuda.h): argument checks and launches.
-#include "kv4_attention.cuh"
+#include "kv4_attention_tc.cuh"
 #include "launch.h"
 
 #include "lunelette_cuda.h"
@@ -174,9 +174,17 @@ LUN_API int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t laye
     }));
 }
 
+// Sequences with more query rows a KV head than this take the block kernel, where
+// there are any and the group fits its tiles.
+constexpr size_t kBlockLeast = 16;
+
 // How a call's keys and rows are split over the GPU.
 struct AttnPlan {
+    bool decode, block;  // which kernels run
+    // decode kernel
     int nt, tile_rows, tiles, split_pages, splits;
+    // block kernel
+    int least, block_tiles, block_split_pages, block_splits;
     size_t part_bytes;
 };
 
@@ -184,49 +192,113 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
                                int type)
 {
     AttnPlan a;
-    const size_t group = query_heads / cache->kv_heads, most = rows->max_count * group;
-    const int lane = type == LUNELETTE_CUDA_FLOAT32 ? 4 : 8;  // rows of an n tile
-    a.nt = most <= (size_t)lane ? 1 : 2;
-    a.tile_rows = lane * a.nt;
-    a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
+    memset(&a, 0, sizeof a);
+    const size_t group = query_heads / cache->kv_heads, part = (cache->head_dim + 2) * sizeof(float);
     const size_t pages = (rows->max_length + kPage - 1) / kPage;
-    const size_t items = rows->sequences * cache->kv_heads * a.tiles, slots = 148 * (a.nt == 1 ? kDecodeCtas : 2);
-    // one wave of CTAs where that leaves each warp a page or more; where there
-    // are more items than CTAs, parts of 16 pages, so that long sequences do not
-    // outlast the short ones
-    size_t splits = slots / (items ? items : 1), per = splits ? (pages + splits - 1) / splits : 16;
-    if (per > 16 && items * 4 > slots) per = 16;
-    a.split_pages = (int)((per + kDecodeWarps - 1) / kDecodeWarps * kDecodeWarps);
-    if (a.split_pages < kDecodeWarps) a.split_pages = kDecodeWarps;
-    a.splits = (int)((pages + a.split_pages - 1) / a.split_pages);
-    if (a.splits < 1) a.splits = 1;
-    a.part_bytes = a.splits == 1 ? 0 : items * a.tile_rows * a.splits * (cache->head_dim + 2) * sizeof(float);
+    size_t most = rows->max_count * group;
+    a.block = most > kBlockLeast && group <= kBlockRows;
+    // a few sequences are not worth the second kernel
+    a.decode = !a.block || rows->sequences > 4;
+    a.least = a.decode ? (int)kBlockLeast : 0;
+    if (a.decode) {
+        if (a.block) most = kBlockLeast;
+        const int lane = type == LUNELETTE_CUDA_FLOAT32 ? 4 : 8;  // rows of an n tile
+        a.nt = most <= (size_t)lane ? 1 : 2;
+        a.tile_rows = lane * a.nt;
+        a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
+        const size_t items = rows->sequences * cache->kv_heads * a.tiles, slots = 148 * (a.nt == 1 ? kDecodeCtas : 2);
+        // one wave of CTAs where that leaves each warp a page or more; where there
+        // are more items than CTAs, parts of 16 pages, so that long sequences do not
+        // outlast the short ones
+        size_t splits = slots / (items ? items : 1), per = splits ? (pages + splits - 1) / splits : 16;
+        if (per > 16 && items * 4 > slots) per = 16;
+        a.split_pages = (int)((per + kDecodeWarps - 1) / kDecodeWarps * kDecodeWarps);
+        if (a.split_pages < kDecodeWarps) a.split_pages = kDecodeWarps;
+        a.splits = (int)((pages + a.split_pages - 1) / a.split_pages);
+        if (a.splits < 1) a.splits = 1;
+        if (a.splits > 1) a.part_bytes = items * a.tile_rows * a.splits * part;
+    }
+    if (a.block) {
+        const size_t tokens = kBlockRows / group, each = (rows->max_count + tokens - 1) / tokens * rows->sequences;
+        const size_t packed = (rows->rows + rows->sequences * (tokens - 1)) / tokens;
+        a.block_tiles = (int)(each < packed ? each : packed);
+        // the splits whose waves of CTAs take the fewest tiles of keys, a CTA's own
+        // steps counted as kOwn of them
+        const size_t ctas = a.block_tiles * cache->kv_heads;
+        size_t best = ~(size_t)0;
+        for (size_t splits = 1; splits <= 16 && splits <= (pages ? pages : 1); splits++) {
+            const size_t kOwn = 6, per = (pages + splits - 1) / splits;
+            const size_t cost = (ctas * splits + 147) / 148 * (per + kOwn) + (splits > 1 ? 3 : 0);
+            if (cost < best) best = cost, a.block_split_pages = (int)per, a.block_splits = (int)splits;
+        }
+        if (a.block_split_pages < 1) a.block_split_pages = 1;
+        if (a.block_splits > 1) a.block_splits = (int)((pages + a.block_split_pages - 1) / a.block_split_pages);
+        const size_t bytes = a.block_splits > 1 ? rows->rows * query_heads * a.block_splits * part : 0;
+        if (bytes > a.part_bytes) a.part_bytes = bytes;  // the kernels run one after the other
+    }
     return a;
+}
+
+static bool valid_heads(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows, size_t query_heads)
+{
+    return query_heads && query_heads <= 4096 && query_heads % cache->kv_heads == 0 &&
+           rows->max_count <= (size_t)(INT_MAX / 2) / (query_heads / cache->kv_heads);
 }
 
 LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
                                                       size_t query_heads)
 {
     bool empty = false;
-    if (!valid_cache(cache, 0) || !valid_rows(rows, &empty) || !query_heads || query_heads > 4096 ||
-        query_heads % cache->kv_heads || empty)
-        return 0;
+    if (!valid_cache(cache, 0) || !valid_rows(rows, &empty) || !valid_heads(cache, rows, query_heads) || empty) return 0;
     const size_t wide = plan_attention(cache, rows, query_heads, LUNELETTE_CUDA_FLOAT32).part_bytes;
     const size_t narrow = plan_attention(cache, rows, query_heads, LUNELETTE_CUDA_FLOAT16).part_bytes;
     return wide > narrow ? wide : narrow;
 }
 
 template <int D, typename T, int NT>
-static cudaError_t launch_decode(const Kv4AttnParams &p, const AttnPlan &a, int sequences, cudaStream_t stream)
+static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_t stream)
 {
     constexpr int smem = Kv4Decode<D, T, NT>::smem;
     auto kernel = kv4_decode_kernel<D, T, NT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    const size_t items = (size_t)sequences * p.cache.heads * a.tiles;
+    p.split_pages = a.split_pages;
+    p.splits = a.splits;
+    p.tiles = a.tiles;
+    p.most = a.block ? a.least : INT_MAX;
+    const size_t items = (size_t)p.rows.sequences * p.cache.heads * a.tiles;
+    if (items > (size_t)INT_MAX / a.splits || items > (size_t)INT_MAX / 8) return cudaErrorInvalidValue;
     e = launch(kernel, dim3((unsigned)(items * a.splits)), dim3(32 * kDecodeWarps), smem, stream, p);
     if (e != cudaSuccess || a.splits == 1) return e;
-    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * ((a.tile_rows + 3) / 4))), dim3(128), 0, stream, p, a.tiles * a.tile_rows);
+    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * ((a.tile_rows + 3) / 4))), dim3(128), 0, stream, p,
+                  a.tiles * a.tile_rows);
+}
+
+template <int D, typename T>
+static cudaError_t launch_block(Kv4AttnParams p, const AttnPlan &a, cudaStream_t stream)
+{
+    constexpr int smem = Kv4BlockLayout<D>::smem;
+    auto kernel = kv4_block_kernel<D, T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    p.split_pages = a.block_split_pages;
+    p.splits = a.block_splits;
+    p.tiles = a.block_tiles;
+    const size_t ctas = (size_t)a.block_tiles * p.cache.heads * a.block_splits;
+    const size_t combines = (size_t)p.rows.rows * ((p.cache.heads * p.group + 3) / 4);
+    if (ctas > INT_MAX || combines > INT_MAX) return cudaErrorInvalidValue;
+    e = launch(kernel, dim3((unsigned)ctas), dim3(kBlockThreads), smem, stream, p, a.least);
+    if (e != cudaSuccess || a.block_splits == 1) return e;
+    return launch(kv4_block_combine_kernel<D, T>, dim3((unsigned)combines), dim3(128), 0, stream, p, a.least);
+}
+
+template <int D, typename T>
+static cudaError_t launch_attention(const Kv4AttnParams &p, const AttnPlan &a, cudaStream_t stream)
+{
+    cudaError_t e = cudaSuccess;
+    if (a.decode) e = a.nt == 1 ? launch_decode<D, T, 1>(p, a, stream) : launch_decode<D, T, 2>(p, a, stream);
+    if (e == cudaSuccess && a.block) e = launch_block<D, T>(p, a, stream);
+    return e;
 }
 
 LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer,
@@ -236,7 +308,7 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
 {
     bool empty = false, wide = true;
     if (!valid_cache(cache, layer) || !valid_rows(rows, &empty) || !valid_type(type)) return -1;
-    if (!query_heads || query_heads > 4096 || query_heads % cache->kv_heads || !(scale - scale == 0.0f)) return -1;
+    if (!valid_heads(cache, rows, query_heads) || !(scale - scale == 0.0f)) return -1;
     const size_t width = query_heads * cache->head_dim;
     if (!valid_tensor(q, q_stride, width, type, empty, &wide) ||
         !valid_tensor(out, out_stride, width, type, empty, &wide) || !aligned(status, 4) || !aligned(workspace, 16))
@@ -244,7 +316,6 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
     if (empty) return 0;
     const AttnPlan a = plan_attention(cache, rows, query_heads, type);
     if (workspace_bytes < a.part_bytes || (a.part_bytes && !workspace)) return -1;
-    if (rows->sequences * cache->kv_heads * a.tiles > (size_t)INT_MAX / a.splits) return -1;
     Kv4AttnParams p;
     memset(&p, 0, sizeof p);
     p.cache = cache_of(cache, layer);
@@ -255,18 +326,12 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
     p.out_stride = out_stride;
     p.group = (int)(query_heads / cache->kv_heads);
     p.scale2 = scale * 1.4426950408889634f;
-    p.split_pages = a.split_pages;
-    p.splits = a.splits;
-    p.tiles = a.tiles;
     p.wide = wide;
     p.part = static_cast<float *>(workspace);
     p.status = status;
-    const int sequences = (int)rows->sequences;
     cudaStream_t st = (cudaStream_t)stream;
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
-        if (cache->head_dim == 128)
-            return a.nt == 1 ? launch_decode<128, T, 1>(p, a, sequences, st) : launch_decode<128, T, 2>(p, a, sequences, st);
-        return a.nt == 1 ? launch_decode<64, T, 1>(p, a, sequences, st) : launch_decode<64, T, 2>(p, a, sequences, st);
+        return cache->head_dim == 128 ? launch_attention<128, T>(p, a, st) : launch_attention<64, T>(p, a, st);
     }));
 }

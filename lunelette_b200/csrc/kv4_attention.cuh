@@ -43,8 +43,11 @@ struct Kv4AttnParams {
     int split_pages;  // pages of a split
     int splits;       // 1: the kernel writes the output itself
     int tiles;        // row tiles of a (sequence, KV head)
+    int most;         // the decode kernel's sequences have at most so many rows a KV head
     bool wide;
-    float *part;      // [sequence][KV head][row of the tiles][split][D + 2]: unnormalised o, m, l
+    // unnormalised o, m, l, D + 2 floats: [sequence][KV head][row of the tiles][split]
+    // of the decode kernel, [row][query head][split] of the block kernel
+    float *part;
     int *status;
 };
 
@@ -150,7 +153,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
         return;
     }
     const int n_rows = q.count * p.group;
-    if (r0 >= n_rows) return;
+    if (r0 >= n_rows || n_rows > p.most) return;
     const int pages = (q.length + kPage - 1) / kPage, first = split * p.split_pages;
     const int last = min(first + p.split_pages, pages);  // this split's pages [first, last)
     if (first >= last && p.splits > 1) return;           // the combine knows how many splits have pages
@@ -503,20 +506,12 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
     }
 }
 
-// One warp per row of a (sequence, KV head): the splits' parts in split order.
-// A block of 4 warps per (sequence, KV head, 4 rows), the rows fastest.
+// One warp: the parts of `splits` splits, in split order, to a row's head.
 template <int D, typename T>
-static __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p, int tile_rows)
+__device__ __forceinline__ void kv4_combine(const Kv4AttnParams &p, const float *part, int splits, int row, int head)
 {
     constexpr int per = D / 32;
-    const int lane = threadIdx.x & 31, fours = (tile_rows + 3) / 4, r = blockIdx.x % fours * 4 + (threadIdx.x >> 5);
-    const int kvh = blockIdx.x / fours % p.cache.heads, s = blockIdx.x / fours / p.cache.heads;
-    pdl_wait();
-    pdl_launch_dependents();
-    const Kv4Sequence q = kv4_sequence(p.rows, s);
-    if (!q.ok || r >= q.count * p.group) return;
-    const int pages = (q.length + kPage - 1) / kPage, splits = (pages + p.split_pages - 1) / p.split_pages;
-    const float *part = p.part + (((size_t)s * p.cache.heads + kvh) * tile_rows + r) * p.splits * (D + 2);
+    const int lane = threadIdx.x & 31;
     float top = -INFINITY, total = 0.0f, x[per] = {};
     for (int i = lane; i < splits; i += 32) top = fmaxf(top, part[(size_t)i * (D + 2) + D]);
     top = warp_max(top);
@@ -542,10 +537,26 @@ static __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p
     }
     total = warp_sum(total);
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    const int token = r / p.group, head = kvh * p.group + r - token * p.group;
-    T *dst = static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + per * lane;
+    T *dst = static_cast<T *>(p.out) + (size_t)row * p.out_stride + (size_t)head * D + per * lane;
 #pragma unroll
     for (int e = 0; e < per; e++) dst[e] = from_float<T>(x[e] * inverse);
+}
+
+// One warp per row of a (sequence, KV head) of the decode kernel's. A block of 4
+// warps takes 4 rows, the rows fastest.
+template <int D, typename T>
+static __global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p, int tile_rows)
+{
+    const int fours = (tile_rows + 3) / 4, r = blockIdx.x % fours * 4 + (threadIdx.x >> 5);
+    const int kvh = blockIdx.x / fours % p.cache.heads, s = blockIdx.x / fours / p.cache.heads;
+    pdl_wait();
+    pdl_launch_dependents();
+    const Kv4Sequence q = kv4_sequence(p.rows, s);
+    if (!q.ok || q.count * p.group > p.most || r >= q.count * p.group) return;
+    const int pages = (q.length + kPage - 1) / kPage, splits = (pages + p.split_pages - 1) / p.split_pages;
+    const int token = r / p.group;
+    kv4_combine<D, T>(p, p.part + (((size_t)s * p.cache.heads + kvh) * tile_rows + r) * p.splits * (D + 2), splits,
+                      q.first + token, kvh * p.group + r - token * p.group);
 }
 
 }  // namespace lun

@@ -376,10 +376,11 @@ def check_rows(torch, name, got, want, spread, weight, total):
     e = 2 * spread[..., None] * 2.0 ** -20 + 2.0 ** -18
     if name != "f32":
         e = e + 2.0 ** -11
-    # The weights' FP16 parts end at 2^-39 of the largest weight (the lo part of 2^14 times it, on FP16's grid
-    # of 2^-24, is off by half of that), and the softmax's sum is at least the largest weight: outputs that
-    # only weights so small reach keep an absolute accuracy of 2^-39 sum |v|.
-    floor = 2.0 ** -39 * total
+    # The weights' FP16 parts end on FP16's grid of 2^-24, off by half of that, after the weights were taken
+    # times 2^14 (decode kernel) or 2^11 (block kernel; the reference maximum is a score the row has seen, so
+    # the largest weight is 2^11 at least there too): 2^-36 of the largest weight, which the softmax's sum
+    # reaches. Outputs that only weights so small make up keep an absolute accuracy of 2^-36 sum |v|.
+    floor = 2.0 ** -36 * total
     bound = weight * e + floor + (np.abs(want) * half_step(torch, name) if name != "f32" else 0) + 1e-30
     if name == "f16":
         bound = bound + 2.0 ** -25  # below 2^-14 FP16 values lie 2^-24 apart, whatever their size: half of that
