@@ -51,7 +51,28 @@ struct Kv4AttnParams {
     int *status;
 };
 
-static __device__ int kv4_error_sink;
+// A bounded wait of one thread on an mbarrier phase. The clock and the abort word
+// are read only after 64 polls: reading %globaltimer on the first poll that fails
+// costs more than most waits here last. False when the CTA gave up.
+__device__ __forceinline__ bool kv4_wait(uint64_t *bar, unsigned parity, volatile int *abort_word)
+{
+    unsigned long long start = 0;
+    for (unsigned spins = 1; !mbar_try_wait(bar, parity); spins++) {
+        if (spins < 64 || (spins & 15u)) continue;
+        const unsigned long long now = wait_clock_ns();
+        if (spins == 64) start = now;
+        if (*abort_word) return false;
+        if (now - start > kWaitLimitNs) {
+            *abort_word = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool kv4_warp_wait(uint64_t *bar, unsigned parity, volatile int *abort_word)
+{
+    return __all_sync(0xffffffffu, kv4_wait(bar, parity, abort_word));
+}
 
 // The softmax's weights are taken times 2^14, and l with them: the largest is
 // 16384, and the FP16 parts of a weight keep 22 bits down to 2^-28 of it, where a
@@ -255,7 +276,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             next(2 * i + 1);
             continue;
         }
-        if (!(ok = warp_wait(&bar[slot], phases >> slot & 1, abort_word, &kv4_error_sink))) break;
+        if (!(ok = kv4_warp_wait(&bar[slot], phases >> slot & 1, abort_word))) break;
         phases ^= 1u << slot;
         const uint8_t *block = buffers + slot * K::half;
         const int p0 = (first + warp + i * W) * kPage;
@@ -366,7 +387,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                     for (int e = 0; e < 4; e++) o[nt][i2][e] *= corr[K::split ? 0 : e & 1];
             }
         }
-        if (!(ok = warp_wait(&bar[slot], phases >> slot & 1, abort_word, &kv4_error_sink))) break;
+        if (!(ok = kv4_warp_wait(&bar[slot], phases >> slot & 1, abort_word))) break;
         phases ^= 1u << slot;
         uint8_t *vblock = buffers + slot * K::half;
         {

@@ -4,45 +4,109 @@
 // One CTA owns 128 query rows (128 / group tokens with the query heads of one KV
 // head) and a page-aligned range of keys, in tiles of 64 (one page):
 //   warp 0      bulk copies of a tile's K half and V half (codes and scales, 4608
-//               bytes each for 128 dims) into two rings of three;
-//   warp 1      allocates tensor memory; one lane issues the MMAs: S = Q K^T into
-//               one of two buffers, O += P V;
-//   warps 2-3   K codes -> d * (c - 8) in FP16 (exact), K-major with the 128-byte
+//               bytes each for 128 dims) into two rings of six, which covers HBM's latency;
+//   warp 1      allocates tensor memory; one lane issues the MMAs: S = Q K^T for two
+//               tiles at once into one of two buffers (with 64 keys an MMA takes as
+//               long as with 128: it waits for Q from tensor memory), O += P V a tile;
+//   warps 2-5   K codes -> d * (c - 8) in FP16 (exact), [key][dim] with the 128-byte
 //               swizzle, two buffers;
-//   warps 4-5   V codes -> the same, transposed, two buffers; values behind the last
-//               position, of a page outside the pool and of NaN scales are zeros;
-//   warps 6-9   a thread per query row: Q into tensor memory once; per tile the
+//   warps 6-9   V codes -> the same (P V takes them as an N-major operand, so nothing is
+//               transposed); values behind the last position, of a page outside the
+//               pool and of NaN scales are zeros;
+//   warps 10-13 a thread per query row: Q into tensor memory once; per tile the
 //               row's 64 scores from tensor memory, causal mask, online softmax,
 //               weights over the scores as the A operand of P V; at the end O / l or
 //               the split's part.
 // FP32 rows go in as FP16 hi + lo parts (two MMAs a product, 22 bits; the cache's
-// side is exact in one part), 16-bit rows as one. Weights are times 2^11, and the
-// running maximum is kept until a tile raises it by more than 2^4, so a weight is at most
-// 2^15 and its parts keep their bits down to 2^-25 of the largest.
+// side is exact in one part), 16-bit rows as one. Weights are times 2^7, and the
+// running maximum is kept until a tile raises it by more than 2^8 (a raise waits for
+// P V and rescales O, up to 2000 cycles; with 2^4 half the tiles had one), so a weight is at
+// most 2^15, and its parts end at 2^-32 of the largest.
 //
 // A code pair leaves the conversion as dims (n, n + 4) of a word, so each 8 dims lie
-// in the order 0 4 1 5 2 6 3 7 in K and, to match, in Q.
+// in the order 0 4 1 5 2 6 3 7 in K and V and, to match, in Q and O.
 //
 // Tensor memory (512 columns, one CTA an SM): Q hi [0, D / 2), Q lo [64, 64 + D / 2), S and P
-// buffers [128, 192) and [192, 256), O [256, 256 + D).
+// buffers of two tiles [128, 256) and [256, 384), O [384, 384 + D).
 #pragma once
 #include "kv4_attention.cuh"
 #include "tcgen05.cuh"
 
 namespace lun {
 
-constexpr int kBlockRows = 128, kBlockThreads = 320, kBlockStages = 3;
-constexpr float kBlockShift = 11.0f, kBlockRaise = 4.0f;
+constexpr int kBlockRows = 128, kBlockThreads = 448, kBlockStages = 6;
+constexpr float kBlockShift = 7.0f, kBlockRaise = 8.0f;
 
 template <int D> struct Kv4BlockLayout {
     static constexpr int half = Kv4Layout<D>::block / 2;
-    static constexpr int tile = kPage * D * 2;                 // FP16 K tile, or V^T tile
-    static constexpr int k_tiles = 0, v_tiles = 2 * tile;      // two buffers each, 1024-byte aligned
-    static constexpr int k_ring = 4 * tile, v_ring = k_ring + kBlockStages * half;
-    static constexpr int bars = v_ring + kBlockStages * half;  // multiple of 8
+    static constexpr int tile = kPage * D * 2;                 // 64 keys of K, or of V, in FP16
+    static constexpr int k_tiles = 0, v_tiles = 4 * tile;      // two buffers of two tiles, and of one
+    static constexpr int k_ring = 6 * tile, v_ring = k_ring + kBlockStages * half;
+    static constexpr int q_stride = D * 4 + 16;  // bytes of a staged row of q, padded against bank conflicts
+    static constexpr int q_rows = v_ring + kBlockStages * half;
+    static constexpr int bars = q_rows + kBlockRows * q_stride;  // multiple of 8
     // more than half of an SM's shared memory: a second CTA would wait for tensor memory
     static constexpr int smem = 1024 + bars + 512 > 118 * 1024 ? 1024 + bars + 512 : 118 * 1024;
 };
+
+// Shared-memory descriptor of an N-major operand with the 128-byte swizzle: rows of
+// 64 elements of N, 8 of them (K) an atom of 1024 bytes, atoms of K 1024 bytes apart
+// (stride byte offset), the next 64 elements of N 8192 bytes on (leading byte offset).
+__device__ __forceinline__ uint64_t sw128_desc_n(uint32_t saddr)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t kIdescNMajorB = 1u << 16;
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Whole warp: 8 consecutive 32-bit columns of this warp's 32 TMEM lanes; tmem_st_wait
+// once for all.
+__device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Two FP32 operations in one instruction, on register pairs.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t p, float &a, float &b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 
 // The row tile `index` of the sequences that the block kernel takes (more than
 // `least` query rows a KV head): its sequence and its place there. A warp asks together.
@@ -81,20 +145,21 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     using L = Kv4Layout<D>;
     using B = Kv4BlockLayout<D>;
     constexpr int G = L::groups, parts = sizeof(T) == 4 ? 2 : 1;
-    constexpr uint32_t q_col = 0, s_col = 128, o_col = 256;
+    constexpr uint32_t q_col = 0, s_col = 128, o_col = 384;
     extern __shared__ __align__(1024) uint8_t kv4_block_raw[];
     const uint32_t raw = smem_u32(kv4_block_raw);
     uint8_t *base = kv4_block_raw + (((raw + 1023u) & ~1023u) - raw);
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + B::bars);
-    uint64_t *k_full = bars, *k_empty = bars + 3, *v_full = bars + 6, *v_empty = bars + 9;       // raw rings
-    uint64_t *k_ready = bars + 12, *k_free = bars + 14, *v_ready = bars + 16, *v_free = bars + 18;  // FP16 tiles
-    uint64_t *s_full = bars + 20, *p_ready = bars + 22, *o_done = bars + 24, *q_ready = bars + 25;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 26);
+    constexpr int N = kBlockStages;
+    uint64_t *k_full = bars, *k_empty = bars + N, *v_full = bars + 2 * N, *v_empty = bars + 3 * N;  // raw rings
+    uint64_t *tiles_at = bars + 4 * N;
+    uint64_t *k_ready = tiles_at, *k_free = tiles_at + 2, *v_ready = tiles_at + 4, *v_free = tiles_at + 6;  // FP16 tiles
+    uint64_t *s_full = tiles_at + 8, *p_ready = tiles_at + 10, *o_done = tiles_at + 12, *q_ready = tiles_at + 13;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 14);
     volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *where = reinterpret_cast<int *>(tmem_slot + 2);    // sequence, place
     int *poison = where + 2;                                // per group of dims: first position with a NaN value
     volatile int *bad = poison + 4;                         // of tile j % 16: its page lies outside the pool
-    int *error = &kv4_error_sink;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, kvh = blockIdx.x / p.splits % p.cache.heads;
     const int index = blockIdx.x / p.splits / p.cache.heads;
@@ -120,16 +185,16 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     if (tiles == 0 && p.splits > 1) return;  // the combine knows which splits have keys
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 3; i++) {
+        for (int i = 0; i < N; i++) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 2);
+            mbar_init(&k_empty[i], 4);
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], 2);
+            mbar_init(&v_empty[i], 4);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&k_ready[i], 2);
+            mbar_init(&k_ready[i], 4);
             mbar_init(&k_free[i], 1);
-            mbar_init(&v_ready[i], 2);
+            mbar_init(&v_ready[i], 4);
             mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 4);
@@ -147,108 +212,128 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        // ---- loads: each ring's next slot as soon as its converters released it
-        if (lane == 0) {
-            const int *table = p.rows.page_tables + s * p.rows.table_stride + k0 / kPage;
-            int ik = 0, iv = 0;
-            unsigned idle = 0;
-            const unsigned long long start = wait_clock_ns();
-            unsigned long long last = start;
-            while ((ik < tiles || iv < tiles) && !*abort_word) {
-                bool progressed = false;
-                if (ik < tiles && (ik < 3 || mbar_test_wait(&k_empty[ik % 3], (ik / 3 - 1) & 1))) {
-                    const uint8_t *block = kv4_block<D>(p.cache, table[ik], kvh);
-                    bad[ik & 15] = !block;
-                    if (block) {
-                        mbar_expect_tx(&k_full[ik % 3], B::half);
-                        bulk_g2s(base + B::k_ring + ik % 3 * B::half, block, B::half, &k_full[ik % 3]);
-                    } else {
-                        kv4_report(p.status, kKv4BadPage);
-                        mbar_arrive(&k_full[ik % 3]);
-                    }
-                    ik++;
-                    progressed = true;
-                }
-                if (iv < ik && (iv < 3 || mbar_test_wait(&v_empty[iv % 3], (iv / 3 - 1) & 1))) {
-                    const uint8_t *block = kv4_block<D>(p.cache, table[iv], kvh);
-                    if (block) {
-                        mbar_expect_tx(&v_full[iv % 3], B::half);
-                        bulk_g2s(base + B::v_ring + iv % 3 * B::half, block + B::half, B::half, &v_full[iv % 3]);
-                    } else {
-                        mbar_arrive(&v_full[iv % 3]);
-                    }
-                    iv++;
-                    progressed = true;
-                }
-                if (progressed) {
-                    idle = 0;
-                    last = wait_clock_ns();
-                } else if ((++idle & 1023u) == 0 && wait_clock_ns() - last > kWaitLimitNs) {
-                    *abort_word = 1;
-                    atomicExch(error, 1);
-                    break;
+        // ---- loads: each ring's next slot as soon as its converters released it. The warp holds
+        // the ids of 64 tiles, so that no copy waits for the page table
+        const int *table = p.rows.page_tables + s * p.rows.table_stride + k0 / kPage;
+        int ids = lane < tiles ? table[lane] : 0, more = lane + 32 < tiles ? table[lane + 32] : 0;
+        int ik = 0, iv = 0;
+        unsigned idle = 0;
+        unsigned long long last = wait_clock_ns();
+        // one half of tile i into slot i % N of a ring
+        auto issue = [&](int i, int offset, uint8_t *ring, uint64_t *full) {
+            const int id = __shfl_sync(0xffffffffu, i & 32 ? more : ids, i & 31);
+            if (lane) return;
+            const uint8_t *block = kv4_block<D>(p.cache, id, kvh);
+            bad[i & 15] = !block;
+            if (block) {
+                mbar_expect_tx(&full[i % N], B::half);
+                bulk_g2s(ring + i % N * B::half, block + offset, B::half, &full[i % N]);
+            } else {
+                kv4_report(p.status, kKv4BadPage);
+                mbar_arrive(&full[i % N]);
+            }
+        };
+        auto released = [&](int i, uint64_t *empty) {
+            return i < N || __any_sync(0xffffffffu, mbar_test_wait(&empty[i % N], (i / N - 1) & 1));
+        };
+        while (iv < tiles && !__any_sync(0xffffffffu, *abort_word)) {
+            bool progressed = false;
+            if (ik < tiles && released(ik, k_empty)) {
+                issue(ik, 0, base + B::k_ring, k_full);
+                ik++;
+                progressed = true;
+            }
+            if (iv < ik && released(iv, v_empty)) {
+                issue(iv, B::half, base + B::v_ring, v_full);
+                iv++;
+                progressed = true;
+                if ((iv & 31) == 0 && iv + 32 < tiles) {  // 32 ids are used up: K is at most a few tiles ahead
+                    const int fetched = iv + 32 + lane < tiles ? table[iv + 32 + lane] : 0;
+                    if (iv & 32) ids = fetched;
+                    else more = fetched;
                 }
             }
-            // every copy issued has landed before the CTA ends
-            for (int j = max(0, ik - 3); j < ik; j++)
-                mbar_wait_bounded(&k_full[j % 3], (j / 3) & 1, abort_word, error, kWaitSpinLimit);
-            for (int j = max(0, iv - 3); j < iv; j++)
-                mbar_wait_bounded(&v_full[j % 3], (j / 3) & 1, abort_word, error, kWaitSpinLimit);
+            if (progressed) {
+                idle = 0;
+                last = wait_clock_ns();
+            } else if ((++idle & 1023u) == 0 && __any_sync(0xffffffffu, wait_clock_ns() - last > kWaitLimitNs)) {
+                *abort_word = 1;
+                break;
+            }
+        }
+        // every copy issued has landed before the CTA ends
+        if (lane == 0) {
+            for (int j = max(0, ik - N); j < ik; j++)
+                kv4_wait(&k_full[j % N], (j / N) & 1, abort_word);
+            for (int j = max(0, iv - N); j < iv; j++)
+                kv4_wait(&v_full[j % N], (j / N) & 1, abort_word);
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issue: S(j) as soon as K(j) is converted, then P V of tile j - 1
-        if (lane == 0 && tiles > 0) {
-            const uint32_t idesc_s = f16_idesc(128, kPage), idesc_o = f16_idesc(128, D);
-            const uint32_t kt = smem_u32(base + B::k_tiles), vt = smem_u32(base + B::v_tiles);
-            bool ok = mbar_wait_bounded(q_ready, 0, abort_word, error, kWaitSpinLimit);
-            for (int j = 0; ok && j <= tiles; j++) {
-                if (j < tiles) {
-                    const int b = j & 1;
-                    if (!(ok = mbar_wait_bounded(&k_ready[b], (j >> 1) & 1, abort_word, error, kWaitSpinLimit))) break;
-                    tc_fence_after();
-                    const uint32_t sd = tmem + s_col + 64u * (uint32_t)b, k = kt + (uint32_t)b * B::tile;
+        // ---- MMA issue: S of the next two tiles ahead of P V of these. The warp runs
+        // the loop together and one lane issues, so that descriptors stay in uniform registers
+        const uint32_t idesc_o = f16_idesc(128, D) | kIdescNMajorB;
+        const uint64_t k_desc = sw128_desc(smem_u32(base + B::k_tiles));
+        const uint64_t v_desc = sw128_desc_n(smem_u32(base + B::v_tiles));
+        const bool leader = elect_one();
+        const int pairs = (tiles + 1) / 2;
+        bool ok = tiles > 0 && kv4_warp_wait(q_ready, 0, abort_word);
+        auto scores = [&](int i) {  // S of tiles 2 i and 2 i + 1
+            const int b = i & 1;
+            if (!kv4_warp_wait(&k_ready[b], (i >> 1) & 1, abort_word)) return false;
+            tc_fence_after();
+            if (leader) {
+                const uint32_t idesc = 2 * i + 1 < tiles ? f16_idesc(128, 2 * kPage) : f16_idesc(128, kPage);
+                const uint32_t sd = tmem + s_col + 128u * (uint32_t)b;
+                const uint64_t k = k_desc + (uint32_t)b * (2 * B::tile >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
+                for (int ks = 0; ks < D / 16; ks++)
 #pragma unroll
-                        for (int part = 0; part < parts; part++)
-                            tc_mma_f16_tmem_a(sd, tmem + q_col + 64u * part + 8u * ks,
-                                              sw128_desc(k + (ks >> 2) * 8192 + (ks & 3) * 32), idesc_s, (ks | part) != 0);
-                    tc_commit(&k_free[b]);
-                    tc_commit(&s_full[b]);
-                }
-                if (j >= 1) {
-                    const int i = j - 1, b = i & 1;
-                    if (!(ok = mbar_wait_bounded(&p_ready[b], (i >> 1) & 1, abort_word, error, kWaitSpinLimit) &&
-                               mbar_wait_bounded(&v_ready[b], (i >> 1) & 1, abort_word, error, kWaitSpinLimit)))
-                        break;
-                    tc_fence_after();
-                    const uint32_t pa = tmem + s_col + 64u * (uint32_t)b, v = vt + (uint32_t)b * B::tile;
-#pragma unroll
-                    for (int ks = 0; ks < kPage / 16; ks++)
-#pragma unroll
-                        for (int part = 0; part < parts; part++)
-                            tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, sw128_desc(v + ks * 32), idesc_o,
-                                              (i | ks | part) != 0);
-                    tc_commit(&v_free[b]);
-                    tc_commit(o_done);
-                }
+                    for (int part = 0; part < parts; part++)
+                        tc_mma_f16_tmem_a(sd, tmem + q_col + 64u * part + 8u * ks,
+                                          k + (((ks >> 2) * 16384 + (ks & 3) * 32) >> 4), idesc, (ks | part) != 0);
+                tc_commit(&k_free[b]);
+                tc_commit(&s_full[b]);
             }
+            __syncwarp();
+            return true;
+        };
+        ok = ok && scores(0);
+        for (int j = 0; ok && j < tiles; j++) {
+            if ((j & 1) == 0 && j / 2 + 1 < pairs && !(ok = scores(j / 2 + 1))) break;
+            const int b = j & 1;
+            if (!(ok = kv4_warp_wait(&p_ready[b], (j >> 1) & 1, abort_word) &&
+                       kv4_warp_wait(&v_ready[b], (j >> 1) & 1, abort_word)))
+                break;
+            tc_fence_after();
+            if (leader) {
+                const uint32_t pa = tmem + s_col + 128u * (uint32_t)(j >> 1 & 1) + 64u * (uint32_t)b;
+                const uint64_t v = v_desc + (uint32_t)b * (B::tile >> 4);
+#pragma unroll
+                for (int ks = 0; ks < kPage / 16; ks++)
+#pragma unroll
+                    for (int part = 0; part < parts; part++)
+                        tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, v + (ks * 2048 >> 4), idesc_o,
+                                          ks || part || j > 0);
+                tc_commit(&v_free[b]);
+                tc_commit(o_done);
+            }
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp < 4) {
+    } else if (warp < 6) {
         // ---- K: a unit is 16 (8 for 64 dims) bytes of a key's row, word j of them is word 4 j + t of the
         // row; keys k and k + 4 share a quarter warp, whose stores then hit every bank once
-        const int ct = threadIdx.x - 64;  // 0..63
+        const int ct = threadIdx.x - 64;  // 0..127
         for (int j = 0; j < tiles; j++) {
-            if (!warp_wait(&k_full[j % 3], (j / 3) & 1, abort_word, error)) break;
-            if (j >= 2 && !warp_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, abort_word, error)) break;
-            const uint8_t *src = base + B::k_ring + j % 3 * B::half;
-            uint8_t *dst = base + B::k_tiles + (j & 1) * B::tile;
+            const int pair = j >> 1, b = pair & 1;
+            if (!kv4_warp_wait(&k_full[j % N], (j / N) & 1, abort_word)) break;
+            if ((j & 1) == 0 && pair >= 2 && !kv4_warp_wait(&k_free[b], ((pair >> 1) - 1) & 1, abort_word)) break;
+            const uint8_t *src = base + B::k_ring + j % N * B::half;
+            uint8_t *dst = base + B::k_tiles + b * 2 * B::tile;
             if (!bad[j & 15]) {
 #pragma unroll
-                for (int it = 0; it < 4; it++) {
-                    const int u = ct + 64 * it, t = u & 3, key = (u >> 5) * 8 + ((u >> 2) & 1) * 4 + ((u >> 3) & 3);
+                for (int it = 0; it < 2; it++) {
+                    const int u = ct + 128 * it, t = u & 3, key = (u >> 5) * 8 + ((u >> 2) & 1) * 4 + ((u >> 3) & 3);
                     uint32_t w[G], d[G / 2];
                     if constexpr (G == 4) {
                         *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(src + key * (D / 2) + 16 * t);
@@ -257,6 +342,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                         *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(src + key * (D / 2) + 8 * t);
                         d[0] = *reinterpret_cast<const uint32_t *>(src + L::k_scale(key, 0));
                     }
+                    const int row = 64 * (j & 1) + key;
 #pragma unroll
                     for (int g = 0; g < G; g++) {
                         const uint32_t d2 = __byte_perm(d[g >> 1], 0, g & 1 ? 0x3232 : 0x1010);
@@ -266,70 +352,60 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                         v.z = kv4_times(kv4_low(w[g] >> 8), d2);
                         v.w = kv4_times(kv4_high(w[g] >> 8), d2);
                         const int at = 4 * g + t;  // word of the row
-                        *reinterpret_cast<uint4 *>(dst + (at >> 3) * 8192 + sw128_offset(key, (at & 7) * 8)) = v;
+                        *reinterpret_cast<uint4 *>(dst + (at >> 3) * 16384 + sw128_offset(row, (at & 7) * 8)) = v;
                     }
                 }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&k_ready[j & 1]);
-                mbar_arrive(&k_empty[j % 3]);
+                mbar_arrive(&k_empty[j % N]);
+                if ((j & 1) || j == tiles - 1) mbar_arrive(&k_ready[b]);
             }
         }
-    } else if (warp < 6) {
-        // ---- V: a unit is word w of 8 keys, stored as 8 dims x 8 keys; lanes start at different
-        // dims, so that a quarter warp's stores hit every bank once
-        const int ct = threadIdx.x - 128;  // 0..63
+    } else if (warp < 10) {
+        // ---- V: a unit is the 4 words of a group of dims of one key; a quarter warp takes 8 keys, whose
+        // stores then hit every bank once
+        const int ct = threadIdx.x - 192;  // 0..127
         for (int j = 0; j < tiles; j++) {
-            if (!warp_wait(&v_full[j % 3], (j / 3) & 1, abort_word, error)) break;
-            if (j >= 2 && !warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, abort_word, error)) break;
-            const uint8_t *src = base + B::v_ring + j % 3 * B::half - B::half;  // v_word and v_scale count from the block
+            if (!kv4_warp_wait(&v_full[j % N], (j / N) & 1, abort_word)) break;
+            if (j >= 2 && !kv4_warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, abort_word)) break;
+            const uint8_t *src = base + B::v_ring + j % N * B::half - B::half;  // v_word and v_scale count from the block
             uint8_t *dst = base + B::v_tiles + (j & 1) * B::tile;
             const int p0 = k0 + j * kPage, valid = bad[j & 15] ? 0 : seen - p0;
-#pragma unroll 1
-            for (int u = ct; u < L::words * 8; u += 64) {
-                const int w = u % L::words, kg = u / L::words, group = w / 4;
-                uint32_t v[8], d2[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint32_t *>(src + L::v_word(8 * kg + i, w));
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = 8 * kg + 2 * i;
-                    d2[i] = *reinterpret_cast<const uint32_t *>(src + L::v_scale(key, group));
-                    if (key >= valid) d2[i] = 0;
-                    else if (key + 1 >= valid) d2[i] &= 0xffffu;
+            for (int it = 0; it < G / 2; it++) {
+                const int u = ct + 128 * it, key = u & 63, g = u >> 6;
+                const uint4 w4 = *reinterpret_cast<const uint4 *>(src + L::v_word(key, 4 * g));
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                uint32_t d = *reinterpret_cast<const uint16_t *>(src + L::v_scale(key, g));
+                if (key >= valid) d = 0;
+                if ((d & 0x7fffu) > 0x7c00u) {
                     // a NaN times a masked row's weight of zero must not reach that row: the rows that
                     // see the position take it at the end
-                    const uint32_t nan = __hneu2_mask(*reinterpret_cast<__half2 *>(&d2[i]), *reinterpret_cast<__half2 *>(&d2[i]));
-                    if (nan) atomicMin(&poison[group], p0 + key + !(nan & 0xffffu));
-                    d2[i] &= ~nan;
+                    atomicMin(&poison[g], p0 + key);
+                    d = 0;
                 }
-                uint32_t lo[4], hi[4];  // nibbles 0..3 and 4..7 of key pairs
+                const uint32_t d2 = d * 0x10001u;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    lo[i] = __byte_perm(v[2 * i], v[2 * i + 1], 0x5410);
-                    hi[i] = __byte_perm(v[2 * i], v[2 * i + 1], 0x7632);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int e = (i + w) & 7, shift = 4 * (e & 3);
-                    uint4 x;
-                    x.x = kv4_times(kv4_low((e & 4 ? hi[0] : lo[0]) >> shift), d2[0]);
-                    x.y = kv4_times(kv4_low((e & 4 ? hi[1] : lo[1]) >> shift), d2[1]);
-                    x.z = kv4_times(kv4_low((e & 4 ? hi[2] : lo[2]) >> shift), d2[2]);
-                    x.w = kv4_times(kv4_low((e & 4 ? hi[3] : lo[3]) >> shift), d2[3]);
-                    *reinterpret_cast<uint4 *>(dst + sw128_offset(8 * w + e, 8 * kg)) = x;
+                    uint4 v;
+                    v.x = kv4_times(kv4_low(w[i]), d2);
+                    v.y = kv4_times(kv4_high(w[i]), d2);
+                    v.z = kv4_times(kv4_low(w[i] >> 8), d2);
+                    v.w = kv4_times(kv4_high(w[i] >> 8), d2);
+                    const int at = 4 * g + i;
+                    *reinterpret_cast<uint4 *>(dst + (at >> 3) * 8192 + sw128_offset(key, (at & 7) * 8)) = v;
                 }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&v_ready[j & 1]);
-                mbar_arrive(&v_empty[j % 3]);
+                mbar_arrive(&v_empty[j % N]);
             }
         }
-        asm volatile("bar.sync 1, 192;" ::: "memory");  // poison[] is complete
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // poison[] is complete
     } else {
         // ---- softmax: a thread is a query row
         const int row = 32 * (warp & 3) + lane, token = row / p.group, head = kvh * p.group + row - token * p.group;
@@ -339,35 +415,58 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         const size_t tensor_row = (size_t)(q.first + t0 + (live ? token : 0));
         float back;
         {
-            const T *src = static_cast<const T *>(p.q) + tensor_row * p.q_stride + (size_t)(live ? head : 0) * D;
+            // the warp's 32 rows of q, copied row by row into shared memory and read back a row a thread
+            // (read directly, the lanes' 32 rows cost 7 us)
+            uint8_t *mine = base + B::q_rows + 32 * (warp & 3) * B::q_stride;
+            if (p.wide) {
+                constexpr int chunks = D * (int)sizeof(T) / 16, step = 32 / chunks;  // of a row; rows at once
+                int of = 32 * (warp & 3) + lane / chunks, tk = of / p.group, h = of - tk * p.group;
+                const T *src = static_cast<const T *>(p.q) + (size_t)(q.first + t0) * p.q_stride +
+                               (size_t)kvh * p.group * D;
+#pragma unroll 4
+                for (int r = lane / chunks; r < 32; r += step) {
+                    const bool in = tk < tokens && t0 + tk < q.count;
+                    const T *at = in ? src + (size_t)tk * p.q_stride + (size_t)h * D : src;
+                    cp_async16(mine + r * B::q_stride + 16 * (lane % chunks),
+                               reinterpret_cast<const uint8_t *>(at) + 16 * (lane % chunks), in);
+                    for (h += step; h >= p.group; h -= p.group) tk++;
+                }
+                cp_async_commit();
+                cp_async_wait_all();
+            } else {
+                const T *src = static_cast<const T *>(p.q) + tensor_row * p.q_stride + (size_t)(live ? head : 0) * D;
+                for (int d = 0; d < D; d++)
+                    reinterpret_cast<T *>(mine + lane * B::q_stride)[d] = live ? src[d] : from_float<T>(0.0f);
+            }
+            __syncwarp();
+            const T *row_q = reinterpret_cast<const T *>(mine + lane * B::q_stride);
             float top = 0.0f;
 #pragma unroll 4
             for (int d = 0; d < D; d += 8) {
                 float x[8];
-                load8(src + d, p.wide, x);
+                load8(row_q + d, true, x);
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
             }
-            float undo;
-            const float f = live ? power_scale(top, undo) : 0.0f;
-            if (!live) undo = 0.0f;
-            back = undo * p.scale2;
+            // a score is (raw sum) * back with back > 0: the scale's sign goes into q, and a
+            // scale of zero becomes one that moves nothing
+            float f = power_scale(top, back);
+            if (p.scale2 < 0.0f) f = -f;
+            back = fmaxf(back * fabsf(p.scale2), 1e-37f);
+#pragma unroll 2
+            for (int d = 0; d < D; d += 16) {
+                uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int d0 = 0; d0 < D; d0 += 64) {
-                uint32_t hi[32], lo[32];
-#pragma unroll
-                for (int w = 0; w < 8; w++) {
+                for (int w = 0; w < 2; w++) {
                     float x[8];
-                    load8(src + d0 + 8 * w, p.wide, x);
+                    load8(row_q + d + 8 * w, true, x);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float a = live ? x[e] * f : 0.0f, b = live ? x[e + 4] * f : 0.0f;
-                        split_half2(a, b, hi[4 * w + e], lo[4 * w + e]);
-                    }
+                    for (int e = 0; e < 4; e++) split_half2(x[e] * f, x[e + 4] * f, hi[4 * w + e], lo[4 * w + e]);
                 }
-                tmem_st32(lane_base + q_col + d0 / 2, hi);
-                if (parts == 2) tmem_st32(lane_base + q_col + 64u + d0 / 2, lo);
+                tmem_st8_async(lane_base + q_col + d / 2, hi);
+                if (parts == 2) tmem_st8_async(lane_base + q_col + 64u + d / 2, lo);
             }
+            tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
@@ -376,30 +475,35 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < tiles; j++) {
-            if (!(ok = warp_wait(&s_full[j & 1], (j >> 1) & 1, abort_word, error))) break;
+            if (!(ok = kv4_warp_wait(&s_full[j >> 1 & 1], (j >> 2) & 1, abort_word))) break;
             tc_fence_after();
-            const uint32_t sb = s_col + 64u * (uint32_t)(j & 1);
+            const uint32_t sb = s_col + 128u * (uint32_t)(j >> 1 & 1) + 64u * (uint32_t)(j & 1);
             uint32_t raw_s[64];
             tmem_ld32(lane_base + sb, *reinterpret_cast<uint32_t(*)[32]>(&raw_s[0]));
             tmem_ld32(lane_base + sb + 32u, *reinterpret_cast<uint32_t(*)[32]>(&raw_s[32]));
             const int p0 = k0 + j * kPage;
-            float x[64], mx = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 64; c++) x[c] = __uint_as_float(raw_s[c]) * back;
+            float *x = reinterpret_cast<float *>(raw_s);
             if (bad[j & 15] || p0 + kPage - 1 > all_see) {
                 const int last = bad[j & 15] ? -1 : limit;
 #pragma unroll
                 for (int c = 0; c < 64; c++) x[c] = p0 + c <= last ? x[c] : -INFINITY;
             }
+            float top0 = x[0], top1 = x[1];
 #pragma unroll
-            for (int c = 0; c < 64; c++) mx = fmaxf(mx, x[c]);
-            // a row without any key yet has O = 0 and l = 0 and just takes the tile's maximum
-            const bool raise = m != -INFINITY && mx > m + kBlockRaise;
-            const float corr = raise ? exp2_fast(m - mx) : 1.0f;
+            for (int c = 2; c < 62; c += 4) {
+                top0 = max3(top0, x[c], x[c + 1]);
+                top1 = max3(top1, x[c + 2], x[c + 3]);
+            }
+            const float mx = max3(fmaxf(top0, top1), x[62], x[63]);
+            // m and mx are raw sums, of which differences are scored, so that the largest weight is 2^0 times
+            // the shift whatever its size. A row without any key yet has O = 0 and l = 0 and just
+            // takes the tile's maximum
+            const bool raise = m != -INFINITY && (mx - m) * back > kBlockRaise;
+            const float corr = raise ? exp2_fast((m - mx) * back) : 1.0f;
             if (m == -INFINITY || raise) m = mx;
             if (__any_sync(0xffffffffu, raise)) {
                 // O's row *= corr once P V of the tile before has landed
-                if (!(ok = warp_wait(o_done, (j - 1) & 1, abort_word, error))) break;
+                if (!(ok = kv4_warp_wait(o_done, (j - 1) & 1, abort_word))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
@@ -411,21 +515,32 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                 }
             }
             l *= corr;
-            const float zero = m == -INFINITY ? 0.0f : m - kBlockShift;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            const float zero = m == -INFINITY ? 0.0f : -m;
+            uint64_t sum = pack2(0.0f, 0.0f);
+            const uint64_t back2 = pack2(back, back), zero2 = pack2(zero, zero), shift2 = pack2(kBlockShift, kBlockShift);
             uint32_t ph[32], pl[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-                const float a = exp2_fast(x[2 * i] - zero), b = exp2_fast(x[2 * i + 1] - zero);
-                sum0 += a;
-                sum1 += b;
+                float a, b;
+                unpack2(fma_f32x2(add_f32x2(pack2(x[2 * i], x[2 * i + 1]), zero2), back2, shift2), a, b);
+                a = exp2_fast(a);
+                b = exp2_fast(b);
+                const uint64_t ab = pack2(a, b);
+                sum = add_f32x2(sum, ab);
                 if (parts == 2) {
-                    split_half2(a, b, ph[i], pl[i]);
+                    // hi: the 11 leading bits, lo: the rest
+                    const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u);
+                    const float hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+                    float la, lb;
+                    unpack2(add_f32x2(ab, pack2(-ha, -hb)), la, lb);
+                    ph[i] = half2_bits(ha, hb);
+                    pl[i] = half2_bits(la, lb);
                 } else {
-                    const __half2 h = __floats2half2_rn(a, b);
-                    ph[i] = *reinterpret_cast<const uint32_t *>(&h);
+                    ph[i] = half2_bits(a, b);
                 }
             }
+            float sum0, sum1;
+            unpack2(sum, sum0, sum1);
             l += sum0 + sum1;
             tmem_st32(lane_base + sb, ph);
             if (parts == 2) tmem_st32(lane_base + sb + 32u, pl);
@@ -433,8 +548,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[j & 1]);
         }
-        if (ok && tiles > 0) ok = warp_wait(o_done, (tiles - 1) & 1, abort_word, error);
-        asm volatile("bar.sync 1, 192;" ::: "memory");
+        if (ok && tiles > 0) ok = kv4_warp_wait(o_done, (tiles - 1) & 1, abort_word);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         if (__all_sync(0xffffffffu, ok && !*abort_word)) {
             tc_fence_after();
             const bool whole = p.splits == 1;
@@ -457,8 +572,9 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                 for (int i = 0; i < 32; i += 8) {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        x[e] = nan ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[i + e]) * inverse;
+                    for (int e = 0; e < 8; e++)  // columns 0 .. 7 are dims 0 4 1 5 2 6 3 7
+                        x[e] = nan ? __uint_as_float(0x7fc00000u)
+                                   : __uint_as_float(o[i + (e & 3) * 2 + (e >> 2)]) * inverse;
                     if (whole) {
                         store8(out + c + i, p.wide, x);
                     } else {
@@ -468,7 +584,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                     }
                 }
             }
-            if (!whole && live) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);
+            if (!whole && live) *reinterpret_cast<float2 *>(part + D) = make_float2(m * back, l);
         }
     }
     tc_fence_before();

@@ -377,10 +377,11 @@ def check_rows(torch, name, got, want, spread, weight, total):
     if name != "f32":
         e = e + 2.0 ** -11
     # The weights' FP16 parts end on FP16's grid of 2^-24, off by half of that, after the weights were taken
-    # times 2^14 (decode kernel) or 2^11 (block kernel; the reference maximum is a score the row has seen, so
-    # the largest weight is 2^11 at least there too): 2^-36 of the largest weight, which the softmax's sum
-    # reaches. Outputs that only weights so small make up keep an absolute accuracy of 2^-36 sum |v|.
-    floor = 2.0 ** -36 * total
+    # times 2^14 (decode kernel) or 2^7 (block kernel; the reference maximum is a score the row has seen, so
+    # the largest weight is 2^7 at least there too): 2^-32 of the largest weight, which the softmax's sum
+    # reaches. Outputs that only weights so small make up keep an absolute accuracy of 2^-32 sum |v|, under
+    # the 2^-24 of FP32 sums in which larger weights take part.
+    floor = 2.0 ** -32 * total
     bound = weight * e + floor + (np.abs(want) * half_step(torch, name) if name != "f32" else 0) + 1e-30
     if name == "f16":
         bound = bound + 2.0 ** -25  # below 2^-14 FP16 values lie 2^-24 apart, whatever their size: half of that
