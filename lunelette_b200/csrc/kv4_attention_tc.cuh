@@ -155,7 +155,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     uint64_t *tiles_at = bars + 4 * N;
     uint64_t *k_ready = tiles_at, *k_free = tiles_at + 2, *v_ready = tiles_at + 4, *v_free = tiles_at + 6;  // FP16 tiles
     uint64_t *s_full = tiles_at + 8, *p_ready = tiles_at + 10, *o_done = tiles_at + 12, *q_ready = tiles_at + 13;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 14);
+    uint64_t *q_full = tiles_at + 14;  // rows of q staged, a barrier a warp
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 18);
     volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *where = reinterpret_cast<int *>(tmem_slot + 2);    // sequence, place
     int *poison = where + 2;                                // per group of dims: first position with a NaN value
@@ -201,6 +202,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         }
         mbar_init(o_done, 1);
         mbar_init(q_ready, 4);
+        for (int i = 0; i < 4; i++) mbar_init(&q_full[i], 1);
         *abort_word = 0;
         for (int i = 0; i < 4; i++) poison[i] = 0x7fffffff;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -415,30 +417,22 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         const size_t tensor_row = (size_t)(q.first + t0 + (live ? token : 0));
         float back;
         {
-            // the warp's 32 rows of q, copied row by row into shared memory and read back a row a thread
-            // (read directly, the lanes' 32 rows cost 7 us)
+            // the warp's rows of q, one bulk copy a row, into shared memory (read directly, a lane's row
+            // a lane, they take 7 us; by 16-byte asynchronous copies, 3.5)
             uint8_t *mine = base + B::q_rows + 32 * (warp & 3) * B::q_stride;
+            const T *src = static_cast<const T *>(p.q) + tensor_row * p.q_stride + (size_t)(live ? head : 0) * D;
+            const unsigned rows_live = __popc(__ballot_sync(0xffffffffu, live));
+            bool landed = true;
             if (p.wide) {
-                constexpr int chunks = D * (int)sizeof(T) / 16, step = 32 / chunks;  // of a row; rows at once
-                int of = 32 * (warp & 3) + lane / chunks, tk = of / p.group, h = of - tk * p.group;
-                const T *src = static_cast<const T *>(p.q) + (size_t)(q.first + t0) * p.q_stride +
-                               (size_t)kvh * p.group * D;
-#pragma unroll 4
-                for (int r = lane / chunks; r < 32; r += step) {
-                    const bool in = tk < tokens && t0 + tk < q.count;
-                    const T *at = in ? src + (size_t)tk * p.q_stride + (size_t)h * D : src;
-                    cp_async16(mine + r * B::q_stride + 16 * (lane % chunks),
-                               reinterpret_cast<const uint8_t *>(at) + 16 * (lane % chunks), in);
-                    for (h += step; h >= p.group; h -= p.group) tk++;
-                }
-                cp_async_commit();
-                cp_async_wait_all();
+                uint64_t *full = &q_full[warp & 3];
+                if (lane == 0) mbar_expect_tx(full, rows_live * (unsigned)(D * sizeof(T)));
+                __syncwarp();
+                if (live) bulk_g2s(mine + lane * B::q_stride, src, D * sizeof(T), full);
+                landed = kv4_warp_wait(full, 0, abort_word);
             } else {
-                const T *src = static_cast<const T *>(p.q) + tensor_row * p.q_stride + (size_t)(live ? head : 0) * D;
-                for (int d = 0; d < D; d++)
-                    reinterpret_cast<T *>(mine + lane * B::q_stride)[d] = live ? src[d] : from_float<T>(0.0f);
+                for (int d = 0; d < D; d++) reinterpret_cast<T *>(mine + lane * B::q_stride)[d] = src[d];
+                __syncwarp();
             }
-            __syncwarp();
             const T *row_q = reinterpret_cast<const T *>(mine + lane * B::q_stride);
             float top = 0.0f;
 #pragma unroll 4
@@ -448,6 +442,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
             }
+            if (!live || !landed) top = 0.0f;
             // a score is (raw sum) * back with back > 0: the scale's sign goes into q, and a
             // scale of zero becomes one that moves nothing
             float f = power_scale(top, back);
@@ -461,7 +456,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                     float x[8];
                     load8(row_q + d + 8 * w, true, x);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) split_half2(x[e] * f, x[e + 4] * f, hi[4 * w + e], lo[4 * w + e]);
+                    for (int e = 0; e < 4; e++)
+                        split_half2(live ? x[e] * f : 0.0f, live ? x[e + 4] * f : 0.0f, hi[4 * w + e], lo[4 * w + e]);
                 }
                 tmem_st8_async(lane_base + q_col + d / 2, hi);
                 if (parts == 2) tmem_st8_async(lane_base + q_col + 64u + d / 2, lo);
