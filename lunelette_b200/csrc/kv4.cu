@@ -95,6 +95,16 @@ template <typename F> cudaError_t by_type(int type, F &&f)
     }
 }
 
+// Rows of a block: as few as one wave of blocks holds, at 64 registers a thread.
+int block_rows_for(size_t rows, unsigned threads)
+{
+    const size_t slots = 148 * (size_t)(threads > 512 ? 1 : 1024 / threads < 32 ? 1024 / threads : 32);
+    const size_t n = (rows + slots - 1) / slots;
+    return (int)(n < kKv4BlockRows ? n : kKv4BlockRows);
+}
+
+unsigned threads_for(size_t work, size_t most) { return (unsigned)(work < most ? (work + 31) / 32 * 32 : most); }
+
 int ok(cudaError_t e) { return e == cudaSuccess ? 0 : -1; }
 
 }  // namespace
@@ -139,10 +149,13 @@ LUN_API int lunelette_cuda_kv4_append(const lunelette_cuda_kv4 *cache, size_t la
     p.sine = rope_sin;
     p.wide = wide;
     p.status = status;
+    // a thread for every 16 dims of a row, up to 512
+    const unsigned threads = threads_for((2 * cache->kv_heads + p.query_heads) * (cache->head_dim / 16), 512);
+    p.block_rows = block_rows_for(rows->rows, threads);
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
         auto kernel = cache->head_dim == 128 ? kv4_append_kernel<128, T> : kv4_append_kernel<64, T>;
-        return launch(kernel, dim3((unsigned)rows->rows), dim3(256), 0, (cudaStream_t)stream, p);
+        return launch(kernel, dim3((unsigned)((rows->rows + p.block_rows - 1) / p.block_rows)), dim3(threads), 0, (cudaStream_t)stream, p);
     }));
 }
 
@@ -165,12 +178,14 @@ LUN_API int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t laye
     p.v = v;
     p.k_stride = k_stride;
     p.v_stride = v_stride;
+    p.block_rows = block_rows_for(rows->rows, 128);
     p.wide = wide;
     p.status = status;
+    const unsigned threads = threads_for(p.block_rows * 2 * cache->kv_heads * (cache->head_dim / 8), 256);  // one a word
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
         auto kernel = cache->head_dim == 128 ? kv4_read_kernel<128, T> : kv4_read_kernel<64, T>;
-        return launch(kernel, dim3((unsigned)rows->rows), dim3(256), 0, (cudaStream_t)stream, p);
+        return launch(kernel, dim3((unsigned)((rows->rows + p.block_rows - 1) / p.block_rows)), dim3(threads), 0, (cudaStream_t)stream, p);
     }));
 }
 
@@ -260,7 +275,7 @@ static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_
 {
     constexpr int smem = Kv4Decode<D, T, NT>::smem;
     auto kernel = kv4_decode_kernel<D, T, NT>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT>>(smem);
     if (e != cudaSuccess) return e;
     p.split_pages = a.split_pages;
     p.splits = a.splits;
@@ -279,7 +294,7 @@ static cudaError_t launch_block(Kv4AttnParams p, const AttnPlan &a, cudaStream_t
 {
     constexpr int smem = Kv4BlockLayout<D>::smem;
     auto kernel = kv4_block_kernel<D, T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = opt_in<kv4_block_kernel<D, T>>(smem);
     if (e != cudaSuccess) return e;
     p.split_pages = a.block_split_pages;
     p.splits = a.block_splits;

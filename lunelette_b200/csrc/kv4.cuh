@@ -62,32 +62,41 @@ struct Kv4Sequence {
     bool ok;
 };
 
-__device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Rows &r, int s)
+__device__ __forceinline__ Kv4Sequence kv4_checked(const Kv4Rows &r, int first, int end, int length)
 {
     Kv4Sequence q;
-    const int end = r.offsets[s + 1];
-    q.first = r.offsets[s];
-    q.length = r.lengths[s];
-    q.count = (int)((unsigned)end - (unsigned)q.first);
-    q.ok = q.first >= 0 && end >= q.first && end <= r.rows && q.count <= r.max_count && q.length >= 0 &&
-           q.length <= r.max_length;
+    q.first = first;
+    q.length = length;
+    q.count = (int)((unsigned)end - (unsigned)first);
+    q.ok = first >= 0 && end >= first && end <= r.rows && q.count <= r.max_count && length >= 0 && length <= r.max_length;
     return q;
 }
+__device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4Rows &r, int s)
+{
+    return kv4_checked(r, r.offsets[s], r.offsets[s + 1], r.lengths[s]);
+}
 
-// The last sequence whose first row is at or before `row` (a whole warp asks
-// together): 32 probes a round, so 1024 sequences take two rounds of loads.
-__device__ __forceinline__ int kv4_sequence_of_row(const Kv4Rows &r, int row)
+// The sequence of a row: the last whose first row is at or before it (a whole warp
+// asks together). Up to 32 sequences are read a lane each, with their lengths, so that
+// one round of loads finds the row's position; more take 32 probes a round first.
+__device__ __forceinline__ Kv4Sequence kv4_sequence_of_row(const Kv4Rows &r, int row, int &s)
 {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = r.sequences;
-    while (n > 1) {
+    while (n > 32) {
         const int step = (n + 31) / 32, i = lane * step;
         const bool before = i < n && (i == 0 || r.offsets[lo + i] <= row);
         const int last = 31 - __clz(__ballot_sync(0xffffffffu, before));
         lo += last * step;
         n = min(step, n - last * step);
     }
-    return lo;
+    const bool in = lane < n;
+    const int first = in ? r.offsets[lo + lane] : 0, end = in ? r.offsets[lo + lane + 1] : 0;
+    const int length = in ? r.lengths[lo + lane] : 0;
+    const int who = 31 - __clz(__ballot_sync(0xffffffffu, in && (lane == 0 || first <= row)));
+    s = lo + who;
+    return kv4_checked(r, __shfl_sync(0xffffffffu, first, who), __shfl_sync(0xffffffffu, end, who),
+                       __shfl_sync(0xffffffffu, length, who));
 }
 
 // The block of (page, head), or nullptr for a page outside the pool.
@@ -101,6 +110,55 @@ __device__ __forceinline__ uint8_t *kv4_block(const Kv4Cache &c, int page, int h
 __device__ __forceinline__ void kv4_report(int *status, int bit)
 {
     if (status) atomicOr(status, bit);
+}
+
+// Where a row lives: a position of -1 where there is nothing to do (a row behind the
+// last sequence, before position 0, of a sequence that breaks its bounds), a page
+// outside the pool as it stands. A warp asks together.
+constexpr int kKv4BlockRows = 8;
+struct Kv4Place {
+    int position, page;
+};
+__device__ __forceinline__ int kv4_position(const Kv4Rows &r, int row, int *status, const int *&table)
+{
+    int s;
+    const Kv4Sequence q = kv4_sequence_of_row(r, row, s);
+    if (!q.ok && status && (threadIdx.x & 31) == 0) kv4_report(status, kKv4BadRows);
+    table = r.page_tables + s * r.table_stride;
+    const bool in = q.ok && row >= q.first && row < q.first + q.count;
+    return in ? max(-1, q.length - q.count + (row - q.first)) : -1;
+}
+// The places of rows row0 .. row0 + n - 1 into shared memory, for the whole block. The pages are on
+// their way when it returns: a barrier later they are there. A single row is looked up by
+// every warp for itself and returned, without a barrier.
+__device__ __forceinline__ Kv4Place kv4_places(const Kv4Rows &r, int pages, int row0, int n, Kv4Place *places, int *status)
+{
+    const int lane = threadIdx.x & 31;
+    const int *table;
+    if (n == 1) {
+        Kv4Place place;
+        place.position = kv4_position(r, row0, threadIdx.x == 0 ? status : nullptr, table);
+        place.page = place.position >= 0 ? table[place.position / kPage] : 0;
+        return place;
+    }
+    int mine = -1;
+    const int *my_table = nullptr;
+    for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
+        const int position = kv4_position(r, row0 + i, status, table);
+        if (lane == 0) places[i].position = position;
+        if (lane == i / (blockDim.x >> 5)) mine = position, my_table = table;
+    }
+    __syncthreads();
+    if (mine >= 0) {
+        const int i = (threadIdx.x >> 5) + lane * (blockDim.x >> 5), page = my_table[mine / kPage];
+        places[i].page = page;
+        if ((unsigned)page >= (unsigned)pages) kv4_report(status, kKv4BadPage);
+    }
+    return places[0];
+}
+__device__ __forceinline__ void kv4_check_page(const Kv4Place &place, int pages, int *status)
+{
+    if (threadIdx.x == 0 && place.position >= 0 && (unsigned)place.page >= (unsigned)pages) kv4_report(status, kKv4BadPage);
 }
 
 // ---- element types ------------------------------------------------------------------
@@ -132,6 +190,29 @@ __device__ __forceinline__ void load8(const T *p, bool wide, float (&x)[8])
     }
 }
 
+// Eight elements as they are, loaded now and converted later.
+template <typename T> struct Raw8 {
+    static constexpr int vectors = sizeof(T) / 2;
+    uint4 u[vectors];
+    __device__ __forceinline__ void load(const T *p, bool wide)
+    {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < vectors; i++) u[i] = reinterpret_cast<const uint4 *>(p)[i];
+        } else {
+            T *e = reinterpret_cast<T *>(u);
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const
+    {
+        const T *e = reinterpret_cast<const T *>(u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_float(e[i]);
+    }
+};
+
 template <typename T>
 __device__ __forceinline__ void store8(T *p, bool wide, const float (&x)[8])
 {
@@ -158,7 +239,8 @@ struct Kv4AppendParams {
     void *q_out;
     int query_heads;  // 0: no q
     const float *cosine, *sine;
-    bool wide;  // every row of k, v, q and q_out starts on 16 bytes
+    int block_rows;  // rows of a block
+    bool wide;       // every row of k, v, q and q_out starts on 16 bytes
     int *status;
 };
 
@@ -179,9 +261,9 @@ __device__ __forceinline__ double kv4_scale(double m)
     return fmin(fmax(d, -8160.0), 8160.0);
 }
 
-// Eight values of a lane -> their word of codes; the four lanes of an aligned
-// quad hold the 32 values of a group. All lanes of the warp call it.
-__device__ __forceinline__ uint32_t kv4_quantise(const double (&r)[8], __half &scale)
+// Eight values of a lane in 64 bits -> their word of codes; the four lanes of an
+// aligned quad hold the 32 values of a group. All lanes of the warp call it.
+__device__ __noinline__ uint32_t kv4_quantise_exactly(const double (&r)[8], float &scale)
 {
     double high = r[0], low = r[0];
     bool finite = true;
@@ -198,8 +280,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(const double (&r)[8], __half &s
     }
     const unsigned quad = 0xfu << (threadIdx.x & 28);
     finite = (__ballot_sync(0xffffffffu, finite) & quad) == quad;
-    const double d = finite ? kv4_scale(high >= -low ? high : low) : kv4_scale(__longlong_as_double(0x7ff8000000000000ll));
-    scale = __float2half_rn((float)d);
+    const double d = kv4_scale(finite ? (high >= -low ? high : low) : __longlong_as_double(0x7ff8000000000000ll));
+    scale = (float)d;
     uint32_t word = 0x88888888u;
     if (finite && d != 0.0) {
         word = 0;
@@ -212,82 +294,180 @@ __device__ __forceinline__ uint32_t kv4_quantise(const double (&r)[8], __half &s
     return word;
 }
 
-// One block per row; D / 16 lanes take one head's row, each 8 dims of the lower
-// half and their 8 rotation partners.
+// x c - y s and y c + x s with one rounding of the products' sum and one of the
+// second product's error: off by 2^-23 of the result at most, whatever cancels.
+__device__ __forceinline__ float kv4_turn(float x, float c, float y, float s)
+{
+    const float t = y * s;
+    return fmaf(x, c, -t) - fmaf(y, s, -t);
+}
+
+// Eight values of a lane in FP32 -> their word of codes as in 64 bits. Values that are
+// `exact` decide everything: a scale is rounded on their bits, and a quotient next to a
+// tie is divided with one rounding, which cannot reach a tie that it is not (d has 8
+// bits, so r / d is off a tie by more than half an ulp or not at all). Values within 2^-22 of
+// themselves leave the group `unsure` where the scale's rounding, its sign or a quotient lies
+// that near a border, about 1 group in 1000. So does, of all, a value that is not finite or
+// a scale on the grid of FP16's smallest steps or past the clamp. The quad's lanes hold a
+// group and agree on its scale.
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&r)[8], bool exact, float &scale, bool &unsure)
+{
+    float high = r[0], low = r[0];
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        high = fmaxf(high, r[e]);
+        low = fminf(low, r[e]);
+        nan = nan || r[e] != r[e];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    }
+    const float m = high >= -low ? high : low, top = fabsf(m);
+    const uint32_t bits = __float_as_uint(m), rest = bits & 0xffffu;
+    // 2^-14 keeps d = m / -8 off the grid of 2^-24, 60000 off the clamp
+    unsure = nan || !(top >= 0x1p-14f && top <= 60000.0f) ||
+             (!exact && (fabsf(high + low) <= top * 0x1p-20f || (rest >= 0x8000u - 8u && rest <= 0x8000u + 8u)));
+    const float d = __uint_as_float((bits + 0x7fffu + (bits >> 16 & 1u)) & 0xffff0000u) * -0.125f;
+    scale = d;
+    const float inverse = __frcp_rn(d);
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float q = r[e] * inverse;
+        float c = rintf(q);
+        if (fabsf(q - c) > 0.4999f) {
+            const float quotient = __fdiv_rn(r[e], d);
+            c = rintf(quotient);
+            unsure = unsure || (!exact && fabsf(quotient - c) > 0.49999f);
+        }
+        word |= (uint32_t)((int)fminf(fmaxf(c, -8.0f), 7.0f) + 8) << (4 * e);
+    }
+    return word;
+}
+
+// A block takes block_rows rows one after the other, with its places and rotations
+// looked up at once and the next values in flight: one row a block waits four round
+// trips to L2 for each (4401 rows of 40 heads of 64 dims: 19 us, of 4 rows 12). D / 16 lanes
+// take one head's row, each 8 dims of the lower half and their 8 rotation partners.
+// Everything is decided as in 64 bits, in FP32 but for the few values next to a border: with
+// FP64 throughout (its conversions run at an eighth of FP32's rate) those rows took 55 us.
 template <int D, typename T>
-static __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p)
+static __global__ void __launch_bounds__(512, 2) kv4_append_kernel(Kv4AppendParams p)
 {
     using L = Kv4Layout<D>;
     constexpr int lanes = D / 16;
-    const int row = blockIdx.x;
+    __shared__ Kv4Place places[kKv4BlockRows];
+    __shared__ __align__(16) float turns[kKv4BlockRows][2][D];  // the positions' cosines and sines
+    const int i = threadIdx.x % lanes, heads = p.cache.heads, all = 2 * heads + p.query_heads, step = blockDim.x / lanes;
+    const int row0 = blockIdx.x * p.block_rows, n = min(p.block_rows, p.rows.rows - row0);
     pdl_wait();
     pdl_launch_dependents();
-    const int s = kv4_sequence_of_row(p.rows, row);
-    const Kv4Sequence q = kv4_sequence(p.rows, s);
-    if (!q.ok) {
-        if (threadIdx.x == 0) kv4_report(p.status, kKv4BadRows);
-        return;
-    }
-    if (row < q.first || row >= q.first + q.count) return;  // behind the last sequence
-    const int position = q.length - q.count + (row - q.first);
-    if (position < 0) return;
-    const int page = p.rows.page_tables[s * p.rows.table_stride + position / kPage], slot = position % kPage;
-    if ((unsigned)page >= (unsigned)p.cache.pages && threadIdx.x == 0) kv4_report(p.status, kKv4BadPage);
-    const int heads = p.cache.heads, all = 2 * heads + p.query_heads;
-    const int i = threadIdx.x % lanes;
-    const float stretch = query_scale(position);
-    for (int h0 = 0; h0 < all; h0 += blockDim.x / lanes) {
-        const int h = h0 + threadIdx.x / lanes;  // K heads, V heads, query heads
-        const bool live = h < all;
+    // K heads, V heads, query heads: a thread's values are h = its first head, h + step, ..., row after row
+    Raw8<T> raw_lo, raw_hi;
+    auto values = [&](int r, int h) {
         const int kind = h < heads ? 0 : h < 2 * heads ? 1 : 2;
-        const int head = live ? h - (kind == 0 ? 0 : kind == 1 ? heads : 2 * heads) : 0;
-        const T *src = static_cast<const T *>(kind == 0 ? p.k : kind == 1 || !live ? p.v : p.q) +
-                       (size_t)row * (kind == 0 ? p.k_stride : kind == 1 || !live ? p.v_stride : p.q_stride) +
-                       (size_t)head * D + 8 * i;
-        float lo[8], hi[8];
-        load8(src, p.wide, lo);
-        load8(src + D / 2, p.wide, hi);
-        double a[8], b[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            a[e] = lo[e];
-            b[e] = hi[e];
+        const T *src = static_cast<const T *>(kind == 0 ? p.k : kind == 1 ? p.v : p.q) +
+                       (size_t)(row0 + r) * (kind == 0 ? p.k_stride : kind == 1 ? p.v_stride : p.q_stride) +
+                       (size_t)(h - min(kind, 2) * heads) * D + 8 * i;
+        return src;
+    };
+    auto fetch = [&](int r, int h) {
+        const T *src = values(r, h);
+        raw_lo.load(src, p.wide);
+        raw_hi.load(src + D / 2, p.wide);
+    };
+    const int h_first = min((int)threadIdx.x / lanes, all - 1);
+    fetch(0, h_first);
+    const Kv4Place first = kv4_places(p.rows, p.cache.pages, row0, n, places, p.status);
+    if (p.cosine) {
+        for (int e = threadIdx.x; e < n * (D / 2); e += blockDim.x) {  // both tables, 4 floats at once
+            const int r = e / (D / 2), d = e % (D / 2), position = r ? places[r].position : first.position;
+            if (position >= 0)
+                reinterpret_cast<float4 *>(turns[r])[d] = reinterpret_cast<const float4 *>(
+                    (d < D / 4 ? p.cosine : p.sine) + (size_t)position * D)[d % (D / 4)];
         }
-        if (kind != 1 && p.cosine) {
-            const float *c = p.cosine + (size_t)position * D + 8 * i, *sn = p.sine + (size_t)position * D + 8 * i;
-            float cl[8], ch[8], sl[8], sh[8];
-            load8(c, true, cl);
-            load8(c + D / 2, true, ch);
-            load8(sn, true, sl);
-            load8(sn + D / 2, true, sh);
-            // products of two 24-bit values are exact in 64 bits: one rounding in each sum
+    }
+    __syncthreads();
+    for (int r = 0; r < n; r++) {
+        const Kv4Place place = n == 1 ? first : places[r];
+        const int position = place.position, slot = position % kPage;
+        for (int h0 = 0; h0 < all; h0 += step) {
+            const int h = h0 + (int)threadIdx.x / lanes;
+            float lo[8], hi[8], a[8], b[8];
+            raw_lo.get(lo);
+            raw_hi.get(hi);
+            if (h0 + step < all) fetch(r, min(h + step, all - 1));
+            else if (r + 1 < n) fetch(r + 1, h_first);
+            if (position < 0) continue;
+            const bool live = h < all, turn = p.cosine && (h < heads || h >= 2 * heads);
+            const float *cl = &turns[r][0][8 * i], *ch = cl + D / 2, *sl = &turns[r][1][8 * i], *sh = sl + D / 2;
+            if (turn) {
+                float c[8], sn[8];
+                load8(cl, true, c);
+                load8(sl, true, sn);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const double x = a[e], y = b[e];
-                a[e] = fma(x, (double)cl[e], -(y * (double)sl[e]));
-                b[e] = fma(y, (double)ch[e], x * (double)sh[e]);
-            }
-        }
-        __half da, db;
-        const uint32_t wa = kv4_quantise(a, da), wb = kv4_quantise(b, db);
-        if (!live) continue;
-        if (kind == 2) {
-            float x[8], y[8];
+                for (int e = 0; e < 8; e++) a[e] = kv4_turn(lo[e], c[e], hi[e], sn[e]);
+                load8(ch, true, c);
+                load8(sh, true, sn);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = (float)a[e] * stretch;
-                y[e] = (float)b[e] * stretch;
+                for (int e = 0; e < 8; e++) b[e] = kv4_turn(hi[e], c[e], -lo[e], sn[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) a[e] = lo[e], b[e] = hi[e];
             }
-            T *dst = static_cast<T *>(p.q_out) + (size_t)row * p.q_out_stride + (size_t)head * D + 8 * i;
-            store8(dst, p.wide, x);
-            store8(dst + D / 2, p.wide, y);
-        } else if (uint8_t *block = kv4_block<D>(p.cache, page, head)) {
+            if (live && h >= 2 * heads) {
+                const float stretch = query_scale(position);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    a[e] *= stretch;
+                    b[e] *= stretch;
+                }
+                T *dst = static_cast<T *>(p.q_out) + (size_t)(row0 + r) * p.q_out_stride + (size_t)(h - 2 * heads) * D + 8 * i;
+                store8(dst, p.wide, a);
+                store8(dst + D / 2, p.wide, b);
+            }
+            const bool cached = h < 2 * heads;
+            if (!__any_sync(0xffffffffu, cached)) continue;
+            if (n == 1) kv4_check_page(place, p.cache.pages, p.status);
+            float da, db;
+            bool unsure_a, unsure_b;
+            uint32_t wa = kv4_quantise(a, !turn, da, unsure_a), wb = kv4_quantise(b, !turn, db, unsure_b);
+            // a group with an unsure value is done again in 64 bits: products of two 24-bit values are exact
+            // there, and each sum has one rounding
+            const unsigned quad = 0xfu << (threadIdx.x & 28);
+            const unsigned again_a = __ballot_sync(0xffffffffu, cached && unsure_a);
+            const unsigned again_b = __ballot_sync(0xffffffffu, cached && unsure_b);
+            if (again_a | again_b) {
+                const T *src = values(r, min(h, all - 1));
+                for (int part = 0; part < 2; part++) {
+                    if (!(part ? again_b : again_a)) continue;
+                    double x64[8];
+                    for (int e = 0; e < 8; e++) {
+                        const double x = to_float(src[e]), y = to_float(src[D / 2 + e]);
+                        if (part == 0) x64[e] = turn ? fma(x, (double)cl[e], -(y * (double)sl[e])) : x;
+                        else x64[e] = turn ? fma(y, (double)ch[e], x * (double)sh[e]) : y;
+                    }
+                    float d;
+                    const uint32_t word = kv4_quantise_exactly(x64, d);
+                    if ((part ? again_b : again_a) & quad) {
+                        if (part) wb = word, db = d;
+                        else wa = word, da = d;
+                    }
+                }
+            }
+            if (!cached) continue;
+            const int v = h >= heads;
+            uint8_t *block = kv4_block<D>(p.cache, place.page, v ? h - heads : h);
+            if (!block) continue;
             const int w = i, w2 = i + L::words / 2, g = i / 4, g2 = g + L::groups / 2;
-            *reinterpret_cast<uint32_t *>(block + (kind ? L::v_word(slot, w) : L::k_word(slot, w))) = wa;
-            *reinterpret_cast<uint32_t *>(block + (kind ? L::v_word(slot, w2) : L::k_word(slot, w2))) = wb;
+            *reinterpret_cast<uint32_t *>(block + (v ? L::v_word(slot, w) : L::k_word(slot, w))) = wa;
+            *reinterpret_cast<uint32_t *>(block + (v ? L::v_word(slot, w2) : L::k_word(slot, w2))) = wb;
             if ((i & 3) == 0) {
-                *reinterpret_cast<__half *>(block + (kind ? L::v_scale(slot, g) : L::k_scale(slot, g))) = da;
-                *reinterpret_cast<__half *>(block + (kind ? L::v_scale(slot, g2) : L::k_scale(slot, g2))) = db;
+                *reinterpret_cast<__half *>(block + (v ? L::v_scale(slot, g) : L::k_scale(slot, g))) = __float2half_rn(da);
+                *reinterpret_cast<__half *>(block + (v ? L::v_scale(slot, g2) : L::k_scale(slot, g2))) = __float2half_rn(db);
             }
         }
     }
@@ -299,47 +479,39 @@ struct Kv4ReadParams {
     Kv4Rows rows;
     void *k, *v;  // either may be nullptr
     size_t k_stride, v_stride;
+    int block_rows;
     bool wide;
     int *status;
 };
 
-// One block per row; a thread takes one word of codes.
+// A block takes block_rows rows, a thread one word of codes at a time.
 template <int D, typename T>
 static __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4ReadParams p)
 {
     using L = Kv4Layout<D>;
-    const int row = blockIdx.x;
+    __shared__ Kv4Place places[kKv4BlockRows];
+    const int heads = p.cache.heads, per = 2 * heads * L::words;
+    const int row0 = blockIdx.x * p.block_rows, n = min(p.block_rows, p.rows.rows - row0);
     pdl_wait();
     pdl_launch_dependents();
-    const int s = kv4_sequence_of_row(p.rows, row);
-    const Kv4Sequence q = kv4_sequence(p.rows, s);
-    if (!q.ok) {
-        if (threadIdx.x == 0) kv4_report(p.status, kKv4BadRows);
-        return;
-    }
-    if (row < q.first || row >= q.first + q.count) return;
-    const int position = q.length - q.count + (row - q.first);
-    if (position < 0) return;
-    const int page = p.rows.page_tables[s * p.rows.table_stride + position / kPage], slot = position % kPage;
-    if ((unsigned)page >= (unsigned)p.cache.pages) {
-        if (threadIdx.x == 0) kv4_report(p.status, kKv4BadPage);
-        return;
-    }
-    const int heads = p.cache.heads;
-    for (int item = threadIdx.x; item < 2 * heads * L::words; item += blockDim.x) {
-        const int w = item % L::words, h = item / L::words;
+    const Kv4Place first = kv4_places(p.rows, p.cache.pages, row0, n, places, p.status);
+    if (n == 1) kv4_check_page(first, p.cache.pages, p.status);
+    else __syncthreads();
+    for (int item = threadIdx.x; item < n * per; item += blockDim.x) {
+        const int r = item / per, rest = item - r * per, w = rest % L::words, h = rest / L::words;
         const bool is_v = h >= heads;
-        const int head = is_v ? h - heads : h;
         T *dst = static_cast<T *>(is_v ? p.v : p.k);
-        if (!dst) continue;
-        const uint8_t *block = kv4_block<D>(p.cache, page, head);
+        const Kv4Place place = n == 1 ? first : places[r];
+        const int position = place.position, slot = position % kPage, head = is_v ? h - heads : h;
+        const uint8_t *block = kv4_block<D>(p.cache, place.page, head);
+        if (position < 0 || !block || !dst) continue;
         const uint32_t word = *reinterpret_cast<const uint32_t *>(block + (is_v ? L::v_word(slot, w) : L::k_word(slot, w)));
         const float d = __half2float(*reinterpret_cast<const __half *>(
             block + (is_v ? L::v_scale(slot, w / 4) : L::k_scale(slot, w / 4))));
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = (float)((int)(word >> (4 * e) & 15u) - 8) * d;
-        store8(dst + (size_t)row * (is_v ? p.v_stride : p.k_stride) + (size_t)head * D + 8 * w, p.wide, x);
+        store8(dst + (size_t)(row0 + r) * (is_v ? p.v_stride : p.k_stride) + (size_t)head * D + 8 * w, p.wide, x);
     }
 }
 

@@ -601,7 +601,8 @@ static __global__ void __launch_bounds__(128) kv4_block_combine_kernel(Kv4AttnPa
     const int row = blockIdx.x / fours, head = blockIdx.x % fours * 4 + (threadIdx.x >> 5);
     pdl_wait();
     pdl_launch_dependents();
-    const Kv4Sequence q = kv4_sequence(p.rows, kv4_sequence_of_row(p.rows, row));
+    int s;
+    const Kv4Sequence q = kv4_sequence_of_row(p.rows, row, s);
     if (!q.ok || row < q.first || row >= q.first + q.count || q.count * p.group <= least || head >= heads) return;
     const int keys = q.length - q.count + (row - q.first) + 1, width = p.split_pages * kPage;
     const int splits = keys > 0 ? (keys + width - 1) / width : 0;

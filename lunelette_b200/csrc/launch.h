@@ -3,6 +3,7 @@
 // (pdl_wait) before touching anything that kernel wrote. LUNELETTE_PDL=0 turns
 // the attribute off for comparisons.
 #pragma once
+#include <atomic>
 #include <cuda_runtime.h>
 #include <stdlib.h>
 
@@ -32,6 +33,24 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args &&>(args)...);
+}
+
+// Dynamic shared memory above 48 KB (and clusters of more than 8 blocks) for a kernel,
+// set once per kernel and device; safe from several threads.
+template <auto Kernel> cudaError_t opt_in(int smem, bool large_clusters = false)
+{
+    static std::atomic<unsigned long long> done[2];  // devices 0..127
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool known = dev >= 0 && dev < 128;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (known && (done[dev >> 6].load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && large_clusters)
+        e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && known) done[dev >> 6].fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 }  // namespace lun

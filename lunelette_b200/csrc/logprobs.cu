@@ -17,8 +17,7 @@ template <typename T, int THREADS> cudaError_t launch_clusters(LogprobParams p, 
 {
     auto kernel = logprobs_kernel<T, THREADS>;
     constexpr int smem = (int)sizeof(LogprobShared<THREADS>);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess && p.parts > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const cudaError_t e = opt_in<logprobs_kernel<T, THREADS>>(smem, true);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((size_t)p.rows * p.parts));

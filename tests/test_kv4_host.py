@@ -184,13 +184,13 @@ def test_stored_values_are_exact_in_fp16():
 def find_sequence(offsets, row):
     """kv4_sequence_of_row of kv4.cuh, lane by lane."""
     lo, n = 0, len(offsets) - 1
-    while n > 1:
+    while n > 32:
         step = (n + 31) // 32
         before = [lane * step < n and (lane == 0 or offsets[lo + lane * step] <= row) for lane in range(32)]
         last = max(i for i in range(32) if before[i])
         lo += last * step
         n = min(step, n - last * step)
-    return lo
+    return lo + max(i for i in range(n) if i == 0 or offsets[lo + i] <= row)
 
 
 def test_row_search_finds_the_sequence_that_holds_the_row():
