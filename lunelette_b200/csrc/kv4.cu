@@ -29,7 +29,7 @@ size_t block_bytes(size_t head_dim) { return head_dim == 128 ? Kv4Layout<128>::b
 bool valid_sizes(size_t layers, size_t pages, size_t kv_heads, size_t head_dim)
 {
     return layers && layers <= 4096 && pages && pages <= INT_MAX / 64 && kv_heads && kv_heads <= 256 &&
-           (head_dim == 64 || head_dim == 128);
+           pages * kv_heads < 0xffffffffu && (head_dim == 64 || head_dim == 128);
 }
 
 bool valid_cache(const lunelette_cuda_kv4 *c, size_t layer)
@@ -196,8 +196,11 @@ constexpr size_t kBlockLeast = 16;
 // How a call's keys and rows are split over the GPU.
 struct AttnPlan {
     bool decode, block;  // which kernels run
-    // decode kernel
-    int nt, tile_rows, tiles, split_pages, splits;
+    // decode kernel: n tiles and rows of a row tile, row tiles of a sequence's KV head, tiles of 16 keys in
+    // a unit of the list, blocks, whether items can have many parts
+    int nt, tile_rows, tiles, keys16, ctas;
+    bool many_parts;
+    size_t items, items_offset;
     // block kernel
     int least, block_tiles, block_split_pages, block_splits;
     size_t part_bytes;
@@ -221,17 +224,15 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
         a.nt = most <= (size_t)lane ? 1 : 2;
         a.tile_rows = lane * a.nt;
         a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
-        const size_t items = rows->sequences * cache->kv_heads * a.tiles, slots = 148 * (a.nt == 1 ? kDecodeCtas : 2);
-        // one wave of CTAs where that leaves each warp a page or more; where there
-        // are more items than CTAs, parts of 16 pages, so that long sequences do not
-        // outlast the short ones
-        size_t splits = slots / (items ? items : 1), per = splits ? (pages + splits - 1) / splits : 16;
-        if (per > 16 && items * 4 > slots) per = 16;
-        a.split_pages = (int)((per + kDecodeWarps - 1) / kDecodeWarps * kDecodeWarps);
-        if (a.split_pages < kDecodeWarps) a.split_pages = kDecodeWarps;
-        a.splits = (int)((pages + a.split_pages - 1) / a.split_pages);
-        if (a.splits < 1) a.splits = 1;
-        if (a.splits > 1) a.part_bytes = items * a.tile_rows * a.splits * part;
+        a.items = rows->sequences * cache->kv_heads * a.tiles;
+        const size_t slots = 148 * (a.nt == 1 ? kDecodeCtas : 2), warps = slots * kDecodeWarps;
+        const size_t tiles16 = (rows->max_length + 15) / 16 * a.items;
+        a.keys16 = tiles16 <= warps ? 1 : 4;
+        const size_t units = a.keys16 == 1 ? tiles16 : pages * a.items, blocks = (units + kDecodeWarps - 1) / kDecodeWarps;
+        a.ctas = (int)(blocks < slots ? blocks ? blocks : 1 : slots);
+        a.many_parts = (size_t)a.ctas > 16 * a.items;
+        a.items_offset = 2 * (size_t)a.ctas * kDecodeWarps * a.tile_rows * part;
+        a.part_bytes = a.items_offset + a.items * sizeof(int2);
     }
     if (a.block) {
         const size_t tokens = kBlockRows / group, each = (rows->max_count + tokens - 1) / tokens * rows->sequences;
@@ -270,23 +271,22 @@ LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *
     return wide > narrow ? wide : narrow;
 }
 
-template <int D, typename T, int NT>
+template <int D, typename T, int NT, int KT>
 static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_t stream)
 {
     constexpr int smem = Kv4Decode<D, T, NT>::smem;
-    auto kernel = kv4_decode_kernel<D, T, NT>;
-    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT>>(smem);
+    auto kernel = kv4_decode_kernel<D, T, NT, KT>;
+    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, KT>>(smem);
     if (e != cudaSuccess) return e;
-    p.split_pages = a.split_pages;
-    p.splits = a.splits;
     p.tiles = a.tiles;
     p.most = a.block ? a.least : INT_MAX;
-    const size_t items = (size_t)p.rows.sequences * p.cache.heads * a.tiles;
-    if (items > (size_t)INT_MAX / a.splits || items > (size_t)INT_MAX / 8) return cudaErrorInvalidValue;
-    e = launch(kernel, dim3((unsigned)(items * a.splits)), dim3(32 * kDecodeWarps), smem, stream, p);
-    if (e != cudaSuccess || a.splits == 1) return e;
-    return launch(kv4_combine_kernel<D, T>, dim3((unsigned)(items * ((a.tile_rows + 3) / 4))), dim3(128), 0, stream, p,
-                  a.tiles * a.tile_rows);
+    p.items = reinterpret_cast<int2 *>(reinterpret_cast<char *>(p.part) + a.items_offset);
+    if (a.items > (size_t)INT_MAX / 64) return cudaErrorInvalidValue;
+    e = launch(kernel, dim3((unsigned)a.ctas), dim3(32 * kDecodeWarps), smem, stream, p);
+    if (e != cudaSuccess) return e;
+    const unsigned rows = (unsigned)(a.items * a.tile_rows);
+    if (a.many_parts) return launch(kv4_combine_kernel<D, T, 8>, dim3(rows), dim3(256), 0, stream, p, a.tile_rows);
+    return launch(kv4_combine_kernel<D, T, 1>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, a.tile_rows);
 }
 
 template <int D, typename T>
@@ -311,7 +311,10 @@ template <int D, typename T>
 static cudaError_t launch_attention(const Kv4AttnParams &p, const AttnPlan &a, cudaStream_t stream)
 {
     cudaError_t e = cudaSuccess;
-    if (a.decode) e = a.nt == 1 ? launch_decode<D, T, 1>(p, a, stream) : launch_decode<D, T, 2>(p, a, stream);
+    if (a.decode) {
+        if (a.keys16 == 1) e = a.nt == 1 ? launch_decode<D, T, 1, 1>(p, a, stream) : launch_decode<D, T, 2, 1>(p, a, stream);
+        else e = a.nt == 1 ? launch_decode<D, T, 1, 4>(p, a, stream) : launch_decode<D, T, 2, 4>(p, a, stream);
+    }
     if (e == cudaSuccess && a.block) e = launch_block<D, T>(p, a, stream);
     return e;
 }

@@ -606,7 +606,8 @@ static __global__ void __launch_bounds__(128) kv4_block_combine_kernel(Kv4AttnPa
     if (!q.ok || row < q.first || row >= q.first + q.count || q.count * p.group <= least || head >= heads) return;
     const int keys = q.length - q.count + (row - q.first) + 1, width = p.split_pages * kPage;
     const int splits = keys > 0 ? (keys + width - 1) / width : 0;
-    kv4_combine<D, T>(p, p.part + ((size_t)row * heads + head) * p.splits * (D + 2), splits, row, head);
+    const float *part = p.part + ((size_t)row * heads + head) * p.splits * (D + 2);
+    kv4_combine<D, T, 1>(p, [&](int i) { return part + (size_t)i * (D + 2); }, splits, row, head);
 }
 
 }  // namespace lun
