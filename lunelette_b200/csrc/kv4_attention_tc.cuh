@@ -154,9 +154,9 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     uint64_t *k_full = bars, *k_empty = bars + N, *v_full = bars + 2 * N, *v_empty = bars + 3 * N;  // raw rings
     uint64_t *tiles_at = bars + 4 * N;
     uint64_t *k_ready = tiles_at, *k_free = tiles_at + 2, *v_ready = tiles_at + 4, *v_free = tiles_at + 6;  // FP16 tiles
-    uint64_t *s_full = tiles_at + 8, *p_ready = tiles_at + 10, *o_done = tiles_at + 12, *q_ready = tiles_at + 13;
-    uint64_t *q_full = tiles_at + 14;  // rows of q staged, a barrier a warp
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 18);
+    uint64_t *s_full = tiles_at + 8, *p_ready = tiles_at + 10, *o_done = tiles_at + 12, *q_ready = tiles_at + 14;
+    uint64_t *q_full = tiles_at + 15;  // rows of q staged, a barrier a warp
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 19);
     volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *where = reinterpret_cast<int *>(tmem_slot + 2);    // sequence, place
     int *poison = where + 2;                                // per group of dims: first position with a NaN value
@@ -199,8 +199,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             mbar_init(&v_free[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 4);
+            mbar_init(&o_done[i], 1);
         }
-        mbar_init(o_done, 1);
         mbar_init(q_ready, 4);
         for (int i = 0; i < 4; i++) mbar_init(&q_full[i], 1);
         *abort_word = 0;
@@ -318,7 +318,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                         tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, v + (ks * 2048 >> 4), idesc_o,
                                           ks || part || j > 0);
                 tc_commit(&v_free[b]);
-                tc_commit(o_done);
+                tc_commit(&o_done[b]);
             }
             __syncwarp();
         }
@@ -499,7 +499,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             if (m == -INFINITY || raise) m = mx;
             if (__any_sync(0xffffffffu, raise)) {
                 // O's row *= corr once P V of the tile before has landed
-                if (!(ok = kv4_warp_wait(o_done, (j - 1) & 1, abort_word))) break;
+                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
@@ -541,10 +541,14 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             tmem_st32(lane_base + sb, ph);
             if (parts == 2) tmem_st32(lane_base + sb + 32u, pl);
             tc_fence_before();
+            // not more than two tiles ahead of P V: a barrier's parity tells only two
+            // phases in a row apart, here of p_ready (whose last one the issuer has then seen) and of
+            // o_done, which is otherwise asked only on a raise and at the end
+            if (j >= 2 && !(ok = kv4_warp_wait(&o_done[j & 1], ((j >> 1) - 1) & 1, abort_word))) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[j & 1]);
         }
-        if (ok && tiles > 0) ok = kv4_warp_wait(o_done, (tiles - 1) & 1, abort_word);
+        if (ok && tiles > 0) ok = kv4_warp_wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1 & 1, abort_word);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (__all_sync(0xffffffffu, ok && !*abort_word)) {
             tc_fence_after();

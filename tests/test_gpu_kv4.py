@@ -102,14 +102,16 @@ class Cache:
             for i in range(c):
                 yield int(self.offsets[s]) + i, s, n - c + i
 
-    def fill(self, rng):
+    def fill(self, rng, ramp=0.0):
         """Random keys and values at every position of every sequence, straight into the host's pool:
-        per sequence [length, heads, dim] of the stored values."""
+        per sequence [length, heads, dim] of the stored values. Keys get `ramp` more from page to page."""
         held = []
         for s, n in enumerate(self.lengths):
             stored = []
             for kind in (0, 1):
                 x = rng.standard_normal((n, self.heads, self.dim)) * np.exp2(rng.integers(-1, 2, (1, self.heads, 1)))
+                if kind == 0:
+                    x = x + ramp * (np.arange(n) // 64)[:, None, None]
                 codes, d = ref.quantise(x)
                 for p in range(n):
                     ref.store(self.host[self.layer], self.dim, self.table[s, p // 64], p % 64, codes[p], d[p], kind)
@@ -377,11 +379,12 @@ def check_rows(torch, name, got, want, spread, weight, total):
     if name != "f32":
         e = e + 2.0 ** -11
     # The weights' FP16 parts end on FP16's grid of 2^-24, off by half of that, after the weights were taken
-    # times 2^14 (decode kernel) or 2^7 (block kernel; the reference maximum is a score the row has seen, so
-    # the largest weight is 2^7 at least there too): 2^-32 of the largest weight, which the softmax's sum
-    # reaches. Outputs that only weights so small make up keep an absolute accuracy of 2^-32 sum |v|, under
-    # the 2^-24 of FP32 sums in which larger weights take part.
-    floor = 2.0 ** -32 * total
+    # times 2^14 or 2^5 (decode kernel, the latter in pages whose scales leave 2^-8..2) or 2^7 (block kernel;
+    # the reference maximum is a score the row has seen, so the largest weight is 2^7 at least there too):
+    # 2^-30 of the largest weight, which the softmax's sum reaches. Outputs that only weights so small make
+    # up keep an absolute accuracy of 2^-30 sum |v|, under the 2^-24 of FP32 sums in which larger weights
+    # take part.
+    floor = 2.0 ** -30 * total
     bound = weight * e + floor + (np.abs(want) * half_step(torch, name) if name != "f32" else 0) + 1e-30
     if name == "f16":
         bound = bound + 2.0 ** -25  # below 2^-14 FP16 values lie 2^-24 apart, whatever their size: half of that
@@ -431,6 +434,41 @@ def test_attention_scale_zero_and_negative_and_large_scores(torch):
     held = c.fill(np.random.default_rng(8))
     for scale in (0.0, -0.125, 2.0):
         attention_check(torch, c, held, "f32", 2, scale, seed=9)
+
+
+@pytest.mark.parametrize("name,dim", [("f32", 128), ("f16", 64)])
+def test_attention_scales_of_all_sizes(torch, name, dim):
+    """Groups from FP16's smallest scales to the largest, mixed within pages and apart."""
+    rng = np.random.default_rng(21)
+    for counts, lengths in (([1, 1, 1], [300, 700, 40]), ([20], [150])):
+        c = Cache(torch, counts, lengths, 2, dim, seed=21)
+        held = []
+        for s, n in enumerate(lengths):
+            stored = []
+            for kind in (0, 1):
+                x = rng.standard_normal((n, 2, dim))
+                if kind == 1:  # pages of one size, and pages of all
+                    size = np.where(np.arange(n) // 64 % 2 == 0, rng.integers(-18, 11, (2, dim // 32, n)),
+                                    rng.integers(-18, 11, (2, dim // 32, 1)))
+                    x = x * np.exp2(np.repeat(np.moveaxis(size, 2, 0), 32, 2))
+                codes, d = ref.quantise(x)
+                for p in range(n):
+                    ref.store(c.host[c.layer], dim, c.table[s, p // 64], p % 64, codes[p], d[p], kind)
+                stored.append(ref.dequantise(codes, d))
+            held.append(stored)
+        c.pool.copy_(torch.from_numpy(c.host.reshape(-1)))
+        attention_check(torch, c, held, name, 2, 0.1, seed=22)
+
+
+@pytest.mark.parametrize("name,dim,heads,group,counts,lengths", [
+    ("f32", 128, 8, 4, [256], [1500]), ("f32", 128, 1, 4, [32], [1000]), ("f16", 64, 2, 5, [100, 3, 40], [900, 700, 1300]),
+    ("f16", 128, 4, 8, [64] * 5, [640] * 5)])
+def test_attention_scores_that_rise_from_page_to_page(torch, name, dim, heads, group, counts, lengths):
+    """Rows whose maximum rises by a lot in every page, among rows whose maximum never does: what
+    is summed up so far is scaled down again and again, while later products are under way."""
+    c = Cache(torch, counts, lengths, heads, dim, seed=30)
+    held = c.fill(np.random.default_rng(31), ramp=8.0)
+    attention_check(torch, c, held, name, group, 0.1, seed=32)
 
 
 def test_attention_q_range(torch):
