@@ -263,8 +263,9 @@ int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t layer, const
  * rotated already and may not overlap out. `workspace` (16-byte aligned, no
  * content expected or kept) holds at least
  * lunelette_cuda_kv4_attention_workspace() bytes for the same sizes; calls that
- * may overlap on the GPU, captured graphs among them, need one each. A
- * deterministic result: the same call gives the same bits. */
+ * may overlap on the GPU, captured graphs among them, need one each. The bounds'
+ * sequences * kv_heads * row tiles * pages stay below 2^31. A deterministic
+ * result: the same call gives the same bits. */
 size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
     size_t query_heads);
 int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,

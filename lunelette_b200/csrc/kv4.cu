@@ -197,8 +197,9 @@ constexpr size_t kBlockLeast = 16;
 struct AttnPlan {
     bool decode, block;  // which kernels run
     // decode kernel: n tiles and rows of a row tile, row tiles of a sequence's KV head, tiles of 16 keys in
-    // a unit of the list, blocks, whether items can have many parts
-    int nt, tile_rows, tiles, keys16, ctas;
+    // a unit, blocks, whether items can have many parts
+    int nt, tile_rows, tiles, ctas;
+    int ranks;  // blocks of an item's cluster; 0: the list
     bool many_parts;
     size_t items, items_offset;
     // block kernel
@@ -225,14 +226,26 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
         a.tile_rows = lane * a.nt;
         a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
         a.items = rows->sequences * cache->kv_heads * a.tiles;
-        const size_t slots = 148 * (a.nt == 1 ? kDecodeCtas : 2), warps = slots * kDecodeWarps;
-        const size_t tiles16 = (rows->max_length + 15) / 16 * a.items;
-        a.keys16 = tiles16 <= warps ? 1 : 4;
-        const size_t units = a.keys16 == 1 ? tiles16 : pages * a.items, blocks = (units + kDecodeWarps - 1) / kDecodeWarps;
-        a.ctas = (int)(blocks < slots ? blocks ? blocks : 1 : slots);
-        a.many_parts = (size_t)a.ctas > 16 * a.items;
-        a.items_offset = 2 * (size_t)a.ctas * kDecodeWarps * a.tile_rows * part;
-        a.part_bytes = a.items_offset + a.items * sizeof(int2);
+        const size_t tiles16 = (rows->max_length + 15) / 16;  // of an item
+        // a cluster an item, of as many blocks as there are SMs and 16 keys a warp, where a
+        // warp's share is a page or less (both sides measured at the kernel). A GPC's SMs hold one
+        // or two clusters of 8: 15 of those ran at once (15 KV heads of 2000 keys 10.3 us, 16
+        // of them 18.9 in two waves, 11.9 by clusters of 4), and one less is counted on.
+        const size_t kClusters8 = 14;
+        size_t ranks = 1;
+        while (ranks < (size_t)kClusterRanks && a.items * ranks * 2 <= (ranks < 4 ? 148 : 8 * kClusters8) &&
+               tiles16 > ranks * kClusterWarps)
+            ranks *= 2;
+        if (tiles16 <= 4 * ranks * kClusterWarps && a.items * ranks <= 2 * 148) {
+            a.ranks = (int)ranks;
+        } else {
+            const size_t slots = 148 * (a.nt == 1 ? kListCtas : 2), units = pages * a.items;
+            const size_t blocks = (units + kListWarps - 1) / kListWarps;
+            a.ctas = (int)(blocks < slots ? blocks ? blocks : 1 : slots);
+            a.many_parts = (size_t)a.ctas > 4 * a.items;
+            a.items_offset = 2 * (size_t)a.ctas * kListWarps * a.tile_rows * part;
+            a.part_bytes = a.items_offset + a.items * sizeof(int2);
+        }
     }
     if (a.block) {
         const size_t tokens = kBlockRows / group, each = (rows->max_count + tokens - 1) / tokens * rows->sequences;
@@ -271,22 +284,30 @@ LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *
     return wide > narrow ? wide : narrow;
 }
 
-template <int D, typename T, int NT, int KT>
+template <int D, typename T, int NT>
 static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_t stream)
 {
-    constexpr int smem = Kv4Decode<D, T, NT>::smem;
-    auto kernel = kv4_decode_kernel<D, T, NT, KT>;
-    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, KT>>(smem);
-    if (e != cudaSuccess) return e;
     p.tiles = a.tiles;
     p.most = a.block ? a.least : INT_MAX;
+    if (a.ranks) {
+        constexpr int smem = Kv4Decode<D, T, NT, kClusterWarps>::smem;
+        const cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kClusterWarps>>(smem);
+        if (e != cudaSuccess) return e;
+        p.ranks = a.ranks;
+        return launch_cluster(kv4_decode_kernel<D, T, NT, kClusterWarps>, dim3((unsigned)(a.items * a.ranks)),
+                              dim3(32 * kClusterWarps), smem, a.ranks, stream, p);
+    }
+    constexpr int smem = Kv4Decode<D, T, NT, kListWarps>::smem;
+    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kListWarps>>(smem);
+    if (e != cudaSuccess) return e;
     p.items = reinterpret_cast<int2 *>(reinterpret_cast<char *>(p.part) + a.items_offset);
-    if (a.items > (size_t)INT_MAX / 64) return cudaErrorInvalidValue;
-    e = launch(kernel, dim3((unsigned)a.ctas), dim3(32 * kDecodeWarps), smem, stream, p);
+    const size_t pages = (size_t)p.rows.max_length / kPage + 1;
+    if (a.items > (size_t)INT_MAX / 64 || a.items * pages > (size_t)INT_MAX) return cudaErrorInvalidValue;
+    e = launch(kv4_decode_kernel<D, T, NT, kListWarps>, dim3((unsigned)a.ctas), dim3(32 * kListWarps), smem, stream, p);
     if (e != cudaSuccess) return e;
     const unsigned rows = (unsigned)(a.items * a.tile_rows);
     if (a.many_parts) return launch(kv4_combine_kernel<D, T, 8>, dim3(rows), dim3(256), 0, stream, p, a.tile_rows);
-    return launch(kv4_combine_kernel<D, T, 1>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, a.tile_rows);
+    return launch(kv4_combine_kernel<D, T, 4>, dim3(rows), dim3(128), 0, stream, p, a.tile_rows);
 }
 
 template <int D, typename T>
@@ -311,10 +332,7 @@ template <int D, typename T>
 static cudaError_t launch_attention(const Kv4AttnParams &p, const AttnPlan &a, cudaStream_t stream)
 {
     cudaError_t e = cudaSuccess;
-    if (a.decode) {
-        if (a.keys16 == 1) e = a.nt == 1 ? launch_decode<D, T, 1, 1>(p, a, stream) : launch_decode<D, T, 2, 1>(p, a, stream);
-        else e = a.nt == 1 ? launch_decode<D, T, 1, 4>(p, a, stream) : launch_decode<D, T, 2, 4>(p, a, stream);
-    }
+    if (a.decode) e = a.nt == 1 ? launch_decode<D, T, 1>(p, a, stream) : launch_decode<D, T, 2>(p, a, stream);
     if (e == cudaSuccess && a.block) e = launch_block<D, T>(p, a, stream);
     return e;
 }

@@ -11,8 +11,15 @@
 // are spread. A warp walks its share with its own ring of half blocks, whatever items
 // it crosses; a whole item is written out, the ends of others leave parts that the
 // combine kernel adds up in order. Where a block's warps share one item (long
-// sequences), they merge first, through shared memory. Where there are fewer pages
-// than a quarter of the warps, a share is counted in 16 keys instead.
+// sequences), they merge first, through shared memory. Where that leaves a warp a page
+// or less (one sequence, or short ones), time is what the steps wait for one another:
+// then a cluster of 1 to 8 blocks takes an item, its warps shares of it in 16 keys, and
+// merges it through distributed shared memory, in one launch (one sequence, 8 KV heads
+// of 4 query heads, FP32: 500 keys 7.9 us by clusters, 11.3 by the list; 4096 keys 12.8
+// by either; 8192 keys 17.8 and 13.2). Clusters of 16 do not all find room at once: 23.9
+// us at 4352 keys. Warps of a block: 8, for 16 take 13.3 us there and 9.2 at 512 keys.
+// Blocks of the list: 4 an SM, 3 slots a warp (3 and 4: 136 us for 130 at four sequences of
+// 131072 keys).
 //
 // The products run on mma.sync m16n8k16 with FP16 operands and FP32 sums: a
 // decode step has 1 to 16 query rows a KV head, so a tcgen05 tile of 128 rows would be
@@ -22,17 +29,22 @@
 // bits of one FP16 are taken (q exact after a power-of-two scaling but for what lies
 // 2^-17 below the row's largest; a weight off by 2^-12 of itself, under the rounding of the
 // output), 8 rows an MMA.
-//   S = K Q^T     A: 16 keys x 16 dims of integers c - 8 straight from the
-//                 codes (exact); a group's sum is scaled by d in FP32 after its
-//                 two MMAs, so K needs no multiplication per element.
-//   O^T = V^T P^T A: 16 dims x 16 keys of d * (c - 8), exact in FP16; B: the
-//                 weights, moved from S's layout by movmatrix.
-// A code becomes FP16 by OR-ing it into the mantissa of 1024 (low nibble of a
-// byte) or of 1024 scaled by 16 (high nibble) and subtracting: both exact.
+// A code needs no arithmetic to become FP16: four bits alone in a half's lowest eight are a
+// subnormal, c * 2^-24 or c * 2^-20, which one AND leaves.
+//   S = K Q^T     A: 16 keys x 16 dims of codes as they are; q is times 2^14 or 2^10 to
+//                 match, -8 sum q is what a group's sum starts from, and it is scaled by d in FP32
+//                 after its two MMAs.
+//   O^T = V^T P^T A: 16 dims x 16 keys of d * (c - 8) * 2^-9, one fused multiply-add from
+//                 the code, whose exact result FP16 holds while 2^-8 <= |d| < 2; a page with
+//                 another d takes two more steps a code. B: the weights, moved from S's layout by
+//                 movmatrix.
 #pragma once
 #include "async.cuh"
 #include "attention.cuh"
 #include "kv4.cuh"
+
+#include <cooperative_groups.h>
+#include <type_traits>
 
 namespace lun {
 
@@ -47,6 +59,7 @@ struct Kv4AttnParams {
     int group;     // query heads per KV head
     float scale2;  // scale * log2 e
     int tiles;     // decode kernel: row tiles of a (sequence, KV head), at most
+    int ranks;     // decode kernel: blocks of an item's cluster
     int most;      // decode kernel: its sequences have at most so many rows a KV head
     int split_pages, splits;  // block kernel: pages of a split; splits, 1: the kernel writes the output itself
     bool wide;
@@ -83,25 +96,25 @@ __device__ __forceinline__ bool kv4_warp_wait(uint64_t *bar, unsigned parity, vo
 // The softmax's weights are taken times 2^14, and l with them: the largest is
 // 16384, and the FP16 parts of a weight keep 22 bits down to 2^-28 of it, where a
 // largest weight of 1 would leave small ones on the 2^-24 grid of FP16's
-// subnormals.
-constexpr float kWeightShift = 14.0f;
+// subnormals. Where V is not times 2^-9, they are 2^9 smaller.
+constexpr float kWeightShift = 14.0f, kValueShift = 9.0f, kValueScale = 512.0f;
 
-#ifndef KV4_SLOTS
-#define KV4_SLOTS 4
-#define KV4_CTAS 3
-#endif
-constexpr int kDecodeWarps = 4, kDecodeSlots = KV4_SLOTS, kDecodeCtas = KV4_CTAS;
+constexpr int kListWarps = 4, kListSlots = 3, kListCtas = 4;  // of a block; of a warp; of an SM
+constexpr int kClusterWarps = 8, kClusterSlots = 4, kClusterRanks = 8;  // of a block; of a warp; blocks at most
 
-template <int D, typename T, int NT> struct Kv4Decode {
+template <int D, typename T, int NT, int W> struct Kv4Decode {
     static constexpr bool split = sizeof(T) == 4;    // hi and lo columns
     static constexpr int lane_rows = split ? 1 : 2;  // query rows of a lane and n tile
     static constexpr int rows = 4 * NT * lane_rows;  // query rows of a tile
-    static constexpr int half = Kv4Layout<D>::block / 2;
-    static constexpr int ring = kDecodeWarps * kDecodeSlots * half;
-    static constexpr int merge = kDecodeWarps * rows * (D + 2) * 4;
+    static constexpr int keys = W > kListWarps ? 16 : 64;  // of a unit
+    static constexpr int slots = W > kListWarps ? kClusterSlots : kListSlots;
+    static constexpr int codes = keys * D / 2;
+    static constexpr int half = codes + keys * 2 * (D / 32);  // K or V of a unit, laid out as in a page
+    static constexpr int ring = W * slots * half;
+    static constexpr int merge = (W + 1) * rows * (D + 2) * 4;  // the warps' parts, the block's
     static constexpr int bars = (ring > merge ? ring : merge);
-    static constexpr int prefix = bars + kDecodeWarps * kDecodeSlots * 8;  // 33 * kDecodeWarps long longs
-    static constexpr int smem = prefix + (32 * kDecodeWarps + 1) * 8 + 16;
+    static constexpr int prefix = bars + W * slots * 8;  // an int a thread, one a warp
+    static constexpr int smem = prefix + 33 * W * 4 + 16;
 };
 
 __device__ __forceinline__ float exp2_fast(float x)  // 2 ulp; 0 below 2^-126
@@ -127,6 +140,14 @@ __device__ __forceinline__ uint32_t kv4_high(uint32_t w)
     // (1024 + 16 c) / 16 - 72
     const __half2 h = __hfma2(*reinterpret_cast<__half2 *>(&r), __half2half2(__ushort_as_half(0x2c00)),
                               __half2half2(__ushort_as_half(0xd480)));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The nibbles alone: c * 2^-24 and c * 2^-20 as FP16 subnormals.
+__device__ __forceinline__ uint32_t kv4_code(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t kv4_code16(uint32_t w) { return w & 0x00f000f0u; }
+__device__ __forceinline__ uint32_t kv4_fma(uint32_t v, __half2 x, __half2 y)
+{
+    const __half2 h = __hfma2(*reinterpret_cast<__half2 *>(&v), x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ uint32_t kv4_times(uint32_t v, uint32_t d)
@@ -157,8 +178,7 @@ __device__ __forceinline__ float power_scale(float x, float &back)
 
 // What the decode kernel does of a sequence: units of KT * 16 keys an item, items.
 struct Kv4Share {
-    int units, tiles;
-    long long all;  // units of all its items
+    int units, tiles, all;  // `all`: units of all its items; the caller bounds their sum by 2^31
 };
 template <int KT, int ROWS>
 __device__ __forceinline__ Kv4Share kv4_share(const Kv4AttnParams &p, const Kv4Sequence &q)
@@ -168,22 +188,26 @@ __device__ __forceinline__ Kv4Share kv4_share(const Kv4AttnParams &p, const Kv4S
     if (!q.ok || rows == 0 || rows > p.most) return w;
     w.units = (q.length + 16 * KT - 1) / (16 * KT);
     w.tiles = (rows + ROWS - 1) / ROWS;
-    w.all = (long long)w.units * p.cache.heads * w.tiles;
+    w.all = w.units * p.cache.heads * w.tiles;
     return w;
 }
 
-// Grid: any number of blocks; items [sequence][KV head][row tile of p.tiles].
-template <int D, typename T, int NT, int KT>
-static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCtas : 2) kv4_decode_kernel(Kv4AttnParams p)
+// Items [sequence][KV head][row tile of p.tiles]. W = kListWarps: any number of blocks
+// share the list. W = kClusterWarps: a cluster per item.
+template <int D, typename T, int NT, int W>
+static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? kListCtas : 2)
+    kv4_decode_kernel(Kv4AttnParams p)
 {
+    namespace cg = cooperative_groups;
     using L = Kv4Layout<D>;
-    using K = Kv4Decode<D, T, NT>;
-    constexpr int G = L::groups, MT = D / 16, RP = K::lane_rows, W = kDecodeWarps, SLOTS = kDecodeSlots;
+    using K = Kv4Decode<D, T, NT, W>;
+    constexpr int G = L::groups, MT = D / 16, RP = K::lane_rows, SLOTS = K::slots, KT = K::keys / 16;
+    constexpr bool cluster = W > kListWarps;
     constexpr int row_bytes = D / 2;
     extern __shared__ __align__(128) uint8_t kv4_smem[];
     uint64_t *bars = reinterpret_cast<uint64_t *>(kv4_smem + K::bars);
-    long long *prefix = reinterpret_cast<long long *>(kv4_smem + K::prefix);  // of 128 runs of sequences
-    volatile int *abort_word = reinterpret_cast<volatile int *>(prefix + 32 * W + 1);
+    int *prefix = reinterpret_cast<int *>(kv4_smem + K::prefix);  // of a warp's 32 runs of sequences; warps' totals
+    volatile int *abort_word = reinterpret_cast<volatile int *>(prefix + 33 * W);
     volatile int *merged_word = abort_word + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t *bar = bars + warp * SLOTS;
@@ -193,69 +217,102 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- this warp's units [u0, u1) of the list
-    const int run = (p.rows.sequences + 32 * W - 1) / (32 * W);  // sequences of a thread
-    {
-        long long sum = 0;
-        for (int i = 0; i < run; i++) {
-            const int s = threadIdx.x * run + i;
-            if (s >= p.rows.sequences) break;
-            const Kv4Sequence q = kv4_sequence(p.rows, s);
-            if (!q.ok && blockIdx.x == 0) kv4_report(p.status, kKv4BadRows);
-            sum += kv4_share<KT, K::rows>(p, q).all;
-        }
-        long long upto = sum;
+    // ---- this warp's units [u0, u1): of the cluster's item, or of the list
+    int s = 0, base = 0, u0 = 0, u1 = 0, me = 0, cluster_item = 0;
+    bool shared_item = cluster;  // whether the block's warps share one item
+    const int ranks = cluster ? p.ranks : 1, rank = cluster ? (int)blockIdx.x % ranks : 0;
+    if constexpr (cluster) {
+        cluster_item = blockIdx.x / ranks;
+        s = cluster_item / p.tiles / p.cache.heads;
+        const Kv4Sequence q = kv4_sequence(p.rows, s);
+        const Kv4Share w = kv4_share<KT, K::rows>(p, q);
+        if (!q.ok && threadIdx.x == 0) kv4_report(p.status, kKv4BadRows);
+        if (cluster_item % p.tiles >= w.tiles) return;  // the whole cluster
+        const int warps = ranks * W;
+        me = rank * W + warp;
+        u0 = w.units / warps * me + w.units % warps * me / warps;
+        u1 = w.units / warps * (me + 1) + w.units % warps * (me + 1) / warps;
+        __syncthreads();
+    } else {
+        const int run = (p.rows.sequences + 32 * W - 1) / (32 * W);  // sequences of a thread
+        int total = 0, before = 0;
+        {
+            int sum = 0;
+            for (int i = 0; i < run; i++) {
+                const int s = threadIdx.x * run + i;
+                if (s >= p.rows.sequences) break;
+                const Kv4Sequence q = kv4_sequence(p.rows, s);
+                if (!q.ok && blockIdx.x == 0) kv4_report(p.status, kKv4BadRows);
+                sum += kv4_share<KT, K::rows>(p, q).all;
+            }
+            int upto = sum;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += other;
-        }
-        if (lane == 31) prefix[32 * W - warp] = upto;  // the warps' totals, for a moment
-        __syncthreads();
-        long long before = 0, total = 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += other;
+            }
+            prefix[threadIdx.x] = upto - sum;
+            if (lane == 31) prefix[32 * W + warp] = upto;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const long long all = prefix[32 * W - w];
-            if (w < warp) before += all;
-            total += all;
+            for (int w = 0; w < W; w++) total += prefix[32 * W + w];
+        }
+        const int warps = min((int)gridDim.x * W, total);
+        me = blockIdx.x * W + warp;
+        if ((int)blockIdx.x * W >= warps) return;
+        const int each = total / warps, more = total % warps;
+        auto share_of = [&](int i) { return i >= warps ? total : each * i + more * i / warps; };
+        u0 = share_of(me);
+        u1 = share_of(me + 1);
+        // the sequence of u0 and its first unit
+        if (u1 > u0) {
+            int k = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) {  // the warp's runs that u0 lies in, then the run
+                const int all = prefix[32 * W + w];
+                if (u0 >= before && u0 < before + all) {
+                    k = 32 * w + 31 - __clz(__ballot_sync(0xffffffffu, before + prefix[32 * w + lane] <= u0));
+                    base = before + prefix[k];
+                }
+                before += all;
+            }
+            s = k * run;
+            for (;;) {
+                const int all = kv4_share<KT, K::rows>(p, kv4_sequence(p.rows, s)).all;
+                if (u0 < base + all) break;
+                base += all;
+                s++;
+            }
+        }
+        // the block's warps share an item if the first one's reaches to the last one's end
+        if (warp == 0 && (int)blockIdx.x * W + W <= warps) {
+            const Kv4Share w = kv4_share<KT, K::rows>(p, kv4_sequence(p.rows, s));
+            const int left = w.units - (u0 - base) % w.units;
+            if (lane == 0) *merged_word = u0 + left >= share_of(me + W);
+        } else if (threadIdx.x == 0) {
+            *merged_word = 0;
         }
         __syncthreads();
-        prefix[threadIdx.x] = before + upto - sum;
-        if (threadIdx.x == 0) prefix[32 * W] = total;
-        __syncthreads();
+        shared_item = *merged_word != 0;
     }
-    const long long total = prefix[32 * W];
-    const long long warps = min((long long)gridDim.x * W, total);
-    const long long me = (long long)blockIdx.x * W + warp;
-    if ((long long)blockIdx.x * W >= warps) return;
-    auto share_of = [&](long long i) { return i >= warps ? total : total / warps * i + total % warps * i / warps; };
-    const long long u0 = share_of(me), u1 = share_of(me + 1);
-    const int n = (int)(u1 - u0);
-    // the sequence of u0 and its first unit
-    int s = 0;
-    long long base = 0;
-    if (n > 0) {
-        int k = -1;
-        for (int i = 0; i < W; i++) {
-            const unsigned at = __ballot_sync(0xffffffffu, prefix[32 * i + lane] <= u0);
-            if (at) k = 32 * i + 31 - __clz(at);
-        }
-        s = k * run;
-        base = prefix[k];
-        for (;;) {
-            const long long all = kv4_share<KT, K::rows>(p, kv4_sequence(p.rows, s)).all;
-            if (u0 < base + all) break;
-            base += all;
-            s++;
-        }
-    }
+    const int n = u1 - u0;
+    const bool merged = shared_item;
     // unit base_i + lane of the list: its block in the layer (or none) and its item
     auto map = [&](int i, uint32_t &block, int &item, int &unit) {
         block = 0xffffffffu;
         item = -1;
         unit = 0;
-        const long long u = u0 + i;
+        const int u = u0 + i;
         if (u >= u1) return;
+        if constexpr (cluster) {
+            const int kvh = cluster_item / p.tiles % p.cache.heads;
+            unit = u;
+            item = cluster_item;
+            const int id = p.rows.page_tables[s * p.rows.table_stride + (KT == 4 ? unit : unit >> 2)];
+            if ((unsigned)id < (unsigned)p.cache.pages) block = (uint32_t)id * (uint32_t)p.cache.heads + kvh;
+            else kv4_report(p.status, kKv4BadPage);
+            return;
+        }
         Kv4Share w;
         for (;;) {
             w = kv4_share<KT, K::rows>(p, kv4_sequence(p.rows, s));
@@ -263,9 +320,8 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             base += w.all;
             s++;
         }
-        const long long rest = u - base;
-        const int of = (int)(rest / w.units), kvh = of / w.tiles;
-        unit = (int)(rest - (long long)of * w.units);
+        const int rest = u - base, of = rest / w.units, kvh = of / w.tiles;
+        unit = rest - of * w.units;
         item = (s * p.cache.heads + kvh) * p.tiles + of - kvh * w.tiles;
         const int id = p.rows.page_tables[s * p.rows.table_stride + (KT == 4 ? unit : unit >> 2)];
         if ((unsigned)id < (unsigned)p.cache.pages) block = (uint32_t)id * (uint32_t)p.cache.heads + kvh;
@@ -292,7 +348,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             if (h & 1) issue_unit++;
         }
         if (lane || id == 0xffffffffu) return;
-        const uint8_t *src = p.cache.layer + (size_t)id * L::block + (h & 1 ? K::half : 0);
+        const uint8_t *src = p.cache.layer + (size_t)id * L::block + (h & 1 ? L::block / 2 : 0);
         uint8_t *dst = buffers + slot * K::half;
         if (KT == 4) {
             mbar_expect_tx(&bar[slot], K::half);
@@ -300,26 +356,17 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
         } else {
             constexpr int codes = 16 * row_bytes, scales = 32 * G;
             mbar_expect_tx(&bar[slot], codes + scales);
-            bulk_g2s(dst + quarter * codes, src + quarter * codes, codes, &bar[slot]);
-            bulk_g2s(dst + L::codes + quarter * scales, src + L::codes + quarter * scales, scales, &bar[slot]);
+            bulk_g2s(dst, src + quarter * codes, codes, &bar[slot]);
+            bulk_g2s(dst + codes, src + L::codes + quarter * scales, scales, &bar[slot]);
         }
     };
 #pragma unroll
     for (int h = 0; h < SLOTS; h++)
         if (h < 2 * n) issue(h, h);
-    // whether the block's warps share one item
-    if (warp == 0) {
-        const Kv4Share all = kv4_share<KT, K::rows>(p, kv4_sequence(p.rows, item_at(0) / p.tiles / p.cache.heads));
-        if (lane == 0)
-            *merged_word = (long long)blockIdx.x * W + W <= warps && u0 + all.units - unit >= share_of(me + W);
-    }
-    __syncthreads();
-    const bool merged = *merged_word != 0;
-
     // byte offsets of the lane's first reads in a half block; 16 keys on are 16 rows on, the swizzle the same
-    const int k_at = g * row_bytes + 4 * G * t, ks_at = L::k_scale(g, 0);
-    const int v_even = L::v_word(2 * t, g * (MT / 4)) - K::half, v_odd = v_even ^ row_bytes;
-    const int vs_at = L::v_scale(2 * t, g * (D / 8) / 32) - K::half;
+    const int k_at = g * row_bytes + 4 * G * t, ks_at = L::k_scale(g, 0) - L::codes + K::codes;
+    const int v_even = L::v_word(2 * t, g * (MT / 4)) - L::block / 2, v_odd = v_even ^ row_bytes;
+    const int vs_at = L::v_scale(2 * t, g * (D / 8) / 32) - L::block / 2 - L::codes + K::codes;
     bool ok = true, ends = false;
     unsigned phases = 0;  // parity of each slot's next wait
     int slot = 0;
@@ -331,6 +378,19 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
     float m[NT][RP], l[NT][RP], o[NT][MT][4];
     int item = 0, begin = 0, r0 = 0, kvh = 0;
     Kv4Sequence q = {0, 0, 0, false};
+    if (cluster) {  // a warp without units has a part too
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int e = 0; e < RP; e++) m[nt][e] = -INFINITY, l[nt][e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < MT; j++) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
+        }
+        item = cluster_item;
+        r0 = item % p.tiles * K::rows;
+        kvh = item / p.tiles % p.cache.heads;
+        q = kv4_sequence(p.rows, s);
+    }
     for (int i = 0; i < n && ok;) {
         // ---- an item
         const bool first_item = i == 0;
@@ -342,7 +402,8 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
         const int n_rows = q.count * p.group, units = (q.length + 16 * KT - 1) / (16 * KT);
         // q as B: column g of n tile nt belongs to row (split: 4 nt + g / 2, part g % 2; else 8 nt + g)
         uint32_t qb[NT][D / 16][2];
-        float back[NT][RP];  // what a score is multiplied with, of the lane's rows 4 nt + t or 8 nt + 2 t + (0, 1)
+        float minus8[NT][G][2];  // -8 sum q of a group, as the products count it, of columns 2 t and 2 t + 1
+        float back[NT][RP];      // what a score is multiplied with, of the lane's rows 4 nt + t or 8 nt + 2 t + (0, 1)
         int limit[NT][RP];   // those rows' last visible position
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -370,14 +431,27 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                 for (int hw = 0; hw < 2; hw++)
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
-                        uint32_t hi, lo;
-                        split_half2(x[j][2 * hw + b] * f, x[j][2 * hw + b + 4] * f, hi, lo);
+                        uint32_t hi, lo;  // low nibbles are 2^-4 of high ones
+                        const float up = b ? 0x1p10f * f : 0x1p14f * f;
+                        split_half2(x[j][2 * hw + b] * up, x[j][2 * hw + b + 4] * up, hi, lo);
                         qb[nt][2 * j + hw][b] = K::split && (g & 1) ? lo : hi;
                     }
 #pragma unroll
+            for (int j = 0; j < G; j++) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int hw = 0; hw < 2; hw++)
+                    sum += (low_half(qb[nt][2 * j + hw][0]) + high_half(qb[nt][2 * j + hw][0])) * -0x1p-21f +
+                           (low_half(qb[nt][2 * j + hw][1]) + high_half(qb[nt][2 * j + hw][1])) * -0x1p-17f;
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                minus8[nt][j][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                minus8[nt][j][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            }
+#pragma unroll
             for (int e = 0; e < RP; e++) {
                 // the row's factors sit in the lanes of its (first) column
-                back[nt][e] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + e)) * p.scale2;
+                back[nt][e] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + e)) * (p.scale2 * 0x1p10f);
                 const int row = r0 + (K::split ? 4 * nt + t : 8 * nt + 2 * t + e);
                 limit[nt][e] = row < n_rows ? q.length - q.count + row / p.group : -1;
                 m[nt][e] = -INFINITY;
@@ -401,9 +475,8 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             }
             if (!(ok = kv4_warp_wait(&bar[slot], phases >> slot & 1, abort_word))) break;
             phases ^= 1u << slot;
-            const int p0 = unit * 16 * KT, tile0 = KT == 4 ? 0 : unit & 3;
-            const uint8_t *block = buffers + slot * K::half + tile0 * 16 * row_bytes;
-            const uint8_t *block_scales = buffers + slot * K::half + tile0 * 32 * G;
+            const int p0 = unit * 16 * KT;
+            const uint8_t *block = buffers + slot * K::half;
             float sc[KT][NT][2][RP];
 #pragma unroll
             for (int tile = 0; tile < KT; tile++) {
@@ -411,7 +484,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
                 uint32_t ka[G], kb[G], da[G / 2], db[G / 2];
-                const uint8_t *row = block + k_at + 16 * tile * row_bytes, *scale = block_scales + ks_at + 32 * G * tile;
+                const uint8_t *row = block + k_at + 16 * tile * row_bytes, *scale = block + ks_at + 32 * G * tile;
                 if constexpr (G == 4) {
                     *reinterpret_cast<uint4 *>(ka) = *reinterpret_cast<const uint4 *>(row);
                     *reinterpret_cast<uint4 *>(kb) = *reinterpret_cast<const uint4 *>(row + 8 * row_bytes);
@@ -425,14 +498,14 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                 }
 #pragma unroll
                 for (int j = 0; j < G; j++) {
-                    const uint32_t a0[4] = {kv4_low(ka[j]), kv4_low(kb[j]), kv4_high(ka[j]), kv4_high(kb[j])};
-                    const uint32_t a1[4] = {kv4_low(ka[j] >> 8), kv4_low(kb[j] >> 8), kv4_high(ka[j] >> 8),
-                                            kv4_high(kb[j] >> 8)};
+                    const uint32_t a0[4] = {kv4_code(ka[j]), kv4_code(kb[j]), kv4_code16(ka[j]), kv4_code16(kb[j])};
+                    const uint32_t a1[4] = {kv4_code(ka[j] >> 8), kv4_code(kb[j] >> 8), kv4_code16(ka[j] >> 8),
+                                            kv4_code16(kb[j] >> 8)};
                     const float d0 = j & 1 ? high_half(da[j >> 1]) : low_half(da[j >> 1]);
                     const float d1 = j & 1 ? high_half(db[j >> 1]) : low_half(db[j >> 1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float c[4] = {minus8[nt][j][0], minus8[nt][j][1], minus8[nt][j][0], minus8[nt][j][1]};
                         mma_16816(c, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
                         mma_16816(c, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
                         acc[nt][0] = fmaf(d0, c[0], acc[nt][0]);
@@ -465,6 +538,65 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                             for (int e = 0; e < RP; e++)
                                 if (p0 + 16 * tile + 8 * k8 + g > limit[nt][e]) sc[tile][nt][k8][e] = -INFINITY;
             }
+            if (!(ok = kv4_warp_wait(&bar[slot], phases >> slot & 1, abort_word))) break;
+            phases ^= 1u << slot;
+            uint8_t *vblock = buffers + slot * K::half;
+            uint8_t *vscales = vblock + K::codes;  // [position / 2][group][position % 2]
+            bool small = true;  // every scale is 0 or 2^-8 <= |d| < 2
+            {
+                constexpr int words = KT * 8 * G, each = (words + 31) / 32;
+                uint32_t *mine = reinterpret_cast<uint32_t *>(vscales) + each * lane, d[each] = {};
+                const bool has = words % 32 == 0 || lane < words;
+                const int valid = q.length - p0;
+                if constexpr (each == 4) *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(mine);
+                else if constexpr (each == 2) *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(mine);
+                else if (has) d[0] = *mine;
+                const __half2 least = __half2half2(__ushort_as_half(0x1c00)), most = __half2half2(__ushort_as_half(0x3fff));
+                // quick: zeros are odd too; exact: they are not
+                auto odd = [&](bool exact) {
+                    __half2 high = __habs2(*reinterpret_cast<__half2 *>(&d[0])), low = high;
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int e = 0; e < each; e++) {
+                        const __half2 x = __habs2(*reinterpret_cast<__half2 *>(&d[e]));
+                        high = __hmax2_nan(high, x);
+                        low = __hmin2(low, x);
+                        if (exact) bad |= __hlt2_mask(x, least) & __hne2_mask(x, __half2half2(__ushort_as_half(0)));
+                    }
+                    bad |= __hgtu2_mask(high, most) | (exact ? 0u : __hlt2_mask(low, least));
+                    return __any_sync(0xffffffffu, has && bad != 0);
+                };
+                if (valid < 16 * KT || odd(false)) {
+                    // scales behind the last position (whatever those slots hold) and NaNs become zeros
+                    // before the MMAs, in which a weight of zero would not keep a NaN away from a row
+                    // that does not see its position; the rows that do see a NaN take it here
+                    for (int key = 0; key < min(valid, 16 * KT); key++) {
+                        const int at = ((key >> 1) * G + g * (D / 8) / 32) * 2 + (key & 1);
+                        const float x = __half2float(reinterpret_cast<const __half *>(vscales)[at]);
+                        if (x != x)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int e = 0; e < RP; e++)
+                                    if (p0 + key <= limit[nt][e])
+#pragma unroll
+                                        for (int j = 0; j < MT; j++) o[nt][j][e] = o[nt][j][2 + e] = x;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < each; e++) {
+                        d[e] &= ~__hneu2_mask(*reinterpret_cast<__half2 *>(&d[e]), *reinterpret_cast<__half2 *>(&d[e]));
+                        const int key = (each * lane + e) / G * 2;
+                        if (key >= valid) d[e] = 0;
+                        else if (key + 1 >= valid) d[e] &= 0xffffu;
+                        if (has) mine[e] = d[e];
+                    }
+                    fence_proxy_async_smem();  // before the slot's next bulk copy
+                    __syncwarp();
+                    small = !odd(true);
+                }
+            }
+            const float shift = small ? kWeightShift : kWeightShift - kValueShift, count = small ? 1.0f : kValueScale;
             uint32_t pb[KT][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -499,7 +631,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                 }
                 // a row without any key yet: exp2(-inf - 0) = 0
 #pragma unroll
-                for (int e = 0; e < RP; e++) zero[e] = m[nt][e] == -INFINITY ? 0.0f : m[nt][e] - kWeightShift;
+                for (int e = 0; e < RP; e++) zero[e] = m[nt][e] == -INFINITY ? 0.0f : m[nt][e] - shift;
 #pragma unroll
                 for (int tile = 0; tile < KT; tile++)
 #pragma unroll
@@ -508,7 +640,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
 #pragma unroll
                         for (int e = 0; e < RP; e++) {
                             w[e] = exp2_fast(sc[tile][nt][k8][e] - zero[e]);
-                            l[nt][e] += w[e];
+                            l[nt][e] = fmaf(w[e], count, l[nt][e]);
                         }
                         __half2 two;
                         if constexpr (K::split) {
@@ -520,90 +652,70 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                         pb[tile][nt][k8] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&two));
                     }
             }
-            if (!(ok = kv4_warp_wait(&bar[slot], phases >> slot & 1, abort_word))) break;
-            phases ^= 1u << slot;
-            uint8_t *vblock = buffers + slot * K::half;
-            uint8_t *vscales = vblock + L::codes + tile0 * 32 * G;  // [position / 2][group][position % 2]
-            {
-                // scales behind the last position (whatever those slots hold) and NaNs become zeros
-                // before the MMAs, in which a weight of zero would not keep a NaN away from a row
-                // that does not see its position; the rows that do see a NaN take it here
-                constexpr int words = KT * 8 * G, each = (words + 31) / 32;
-                uint32_t *mine = reinterpret_cast<uint32_t *>(vscales) + lane;
-                uint32_t d[each], nan = 0;
-                const int valid = q.length - p0;
+            auto values = [&](auto fused) {
 #pragma unroll
-                for (int e = 0; e < each; e++) {
-                    d[e] = words % 32 == 0 || lane + 32 * e < words ? mine[32 * e] : 0;
-                    nan |= __hneu2_mask(*reinterpret_cast<__half2 *>(&d[e]), *reinterpret_cast<__half2 *>(&d[e]));
-                }
-                if (valid < 16 * KT || __any_sync(0xffffffffu, nan != 0)) {
-                    for (int key = 0; key < min(valid, 16 * KT); key++) {
-                        const int at = ((key >> 1) * G + g * (D / 8) / 32) * 2 + (key & 1);
-                        const float x = __half2float(reinterpret_cast<const __half *>(vscales)[at]);
-                        if (x != x)
+                for (int tile = 0; tile < KT; tile++) {
+                    uint32_t d2[2], v[4][MT / 4];
+                    const uint8_t *rows16 = vblock + 16 * tile * row_bytes;
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
+                    for (int e = 0; e < 2; e++) {
+                        d2[e] = *reinterpret_cast<const uint32_t *>(vblock + vs_at + (16 * tile + 8 * e) * 2 * G);
 #pragma unroll
-                                for (int e = 0; e < RP; e++)
-                                    if (p0 + key <= limit[nt][e])
-#pragma unroll
-                                        for (int j = 0; j < MT; j++) o[nt][j][e] = o[nt][j][2 + e] = x;
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < each; e++) {
-                        d[e] &= ~__hneu2_mask(*reinterpret_cast<__half2 *>(&d[e]), *reinterpret_cast<__half2 *>(&d[e]));
-                        const int key = (lane + 32 * e) / G * 2;
-                        if (key >= valid) d[e] = 0;
-                        else if (key + 1 >= valid) d[e] &= 0xffffu;
-                        if (words % 32 == 0 || lane + 32 * e < words) mine[32 * e] = d[e];
-                    }
-                    fence_proxy_async_smem();  // before the slot's next bulk copy
-                    __syncwarp();
-                }
-            }
-#pragma unroll
-            for (int tile = 0; tile < KT; tile++) {
-                uint32_t d2[2], v[4][MT / 4];
-                const uint8_t *rows16 = vblock + 16 * (tile0 + tile) * row_bytes;
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    d2[e] = *reinterpret_cast<const uint32_t *>(vblock + vs_at + (16 * (tile0 + tile) + 8 * e) * 2 * G);
-#pragma unroll
-                    for (int odd = 0; odd < 2; odd++) {
-                        const uint8_t *at = rows16 + (odd ? v_odd : v_even) + 8 * e * row_bytes;
-                        if constexpr (MT == 8) *reinterpret_cast<uint2 *>(v[2 * e + odd]) = *reinterpret_cast<const uint2 *>(at);
-                        else v[2 * e + odd][0] = *reinterpret_cast<const uint32_t *>(at);
-                    }
-                }
-#pragma unroll
-                for (int w = 0; w < MT / 4; w++)
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        const uint32_t x0 = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
-                        const uint32_t x1 = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
-#pragma unroll
-                        for (int two = 0; two < 2; two++) {
-                            const uint32_t y0 = two ? x0 >> 8 : x0, y1 = two ? x1 >> 8 : x1;
-                            const uint32_t a[4] = {kv4_times(kv4_low(y0), d2[0]), kv4_times(kv4_high(y0), d2[0]),
-                                                   kv4_times(kv4_low(y1), d2[1]), kv4_times(kv4_high(y1), d2[1])};
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-                                mma_16816(o[nt][4 * w + 2 * half + two], a, pb[tile][nt][0], pb[tile][nt][1]);
+                        for (int odd = 0; odd < 2; odd++) {
+                            const uint8_t *at = rows16 + (odd ? v_odd : v_even) + 8 * e * row_bytes;
+                            if constexpr (MT == 8) *reinterpret_cast<uint2 *>(v[2 * e + odd]) = *reinterpret_cast<const uint2 *>(at);
+                            else v[2 * e + odd][0] = *reinterpret_cast<const uint32_t *>(at);
                         }
                     }
-            }
+                    // c 2^-24 (d 2^15) - d 2^-6 = d (c - 8) 2^-9, of a high nibble from c 2^-20
+                    __half2 x[2], x16[2], y[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const __half2 d = *reinterpret_cast<__half2 *>(&d2[e]);
+                        x[e] = __hmul2(d, __half2half2(__ushort_as_half(0x7800)));    // 2^15
+                        x16[e] = __hmul2(d, __half2half2(__ushort_as_half(0x6800)));  // 2^11
+                        y[e] = __hmul2(d, __half2half2(__ushort_as_half(0xa400)));    // -2^-6
+                    }
+#pragma unroll
+                    for (int w = 0; w < MT / 4; w++)
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const uint32_t x0 = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+                            const uint32_t x1 = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                            for (int two = 0; two < 2; two++) {
+                                const uint32_t y0 = two ? x0 >> 8 : x0, y1 = two ? x1 >> 8 : x1;
+                                uint32_t a[4];
+                                if constexpr (decltype(fused)::value) {
+                                    a[0] = kv4_fma(kv4_code(y0), x[0], y[0]);
+                                    a[1] = kv4_fma(kv4_code16(y0), x16[0], y[0]);
+                                    a[2] = kv4_fma(kv4_code(y1), x[1], y[1]);
+                                    a[3] = kv4_fma(kv4_code16(y1), x16[1], y[1]);
+                                } else {
+                                    a[0] = kv4_times(kv4_low(y0), d2[0]);
+                                    a[1] = kv4_times(kv4_high(y0), d2[0]);
+                                    a[2] = kv4_times(kv4_low(y1), d2[1]);
+                                    a[3] = kv4_times(kv4_high(y1), d2[1]);
+                                }
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++)
+                                    mma_16816(o[nt][4 * w + 2 * half + two], a, pb[tile][nt][0], pb[tile][nt][1]);
+                            }
+                        }
+                }
+            };
+            if (small) values(std::true_type());
+            else values(std::false_type());
             next(2 * i + 1);
         } while (unit++, ++i < n && item_at(i) == item);
         ends = unit == units;
         if (ok && !merged) {
             // the item's end in this warp: the output where all of it was, else a part
             const bool whole = begin == 0 && ends;
-            const int at = 2 * (int)me + (first_item ? 0 : 1);
+            const int at = 2 * me + (first_item ? 0 : 1);
             if (lane == 0) {
                 if (begin == 0) p.items[item].x = whole ? -1 : at;
-                if (ends && !whole) p.items[item].y = (int)me;
+                if (ends && !whole) p.items[item].y = me;
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -615,7 +727,7 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                     const int r = K::split ? 4 * nt + t : 8 * nt + 2 * t + e;
                     if (r0 + r >= n_rows) continue;
-                    const float inverse = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const float inverse = !whole ? kValueScale : sum == 0.0f ? 0.0f : kValueScale / sum;
                     const int token = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) - token * p.group;
                     T *out = static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + g * MT * 2;
                     float *part = p.part + ((size_t)at * K::rows + r) * (D + 2);
@@ -646,11 +758,8 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             for (unsigned spin = 0; spin < 1024 && !mbar_test_wait(&bar[i], phases >> i & 1); spin++) __nanosleep(500);
     }
     __syncthreads();
-    if (*abort_word) {
-        if (threadIdx.x == 0) kv4_report(p.status, kKv4Timeout);
-        return;
-    }
-    if (!merged) return;
+    if (*abort_word && threadIdx.x == 0) kv4_report(p.status, kKv4Timeout);
+    if (!cluster && (*abort_word || !merged)) return;  // a cluster goes on together
     // ---- merge the warps' parts of the block's one item, in warp order
     float *mo = reinterpret_cast<float *>(kv4_smem), *ml = mo + W * K::rows * D;
 #pragma unroll
@@ -666,28 +775,38 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
 #pragma unroll
             for (int i = 0; i < MT; i++)
                 *reinterpret_cast<float2 *>(dst + 2 * i) =
-                    K::split ? make_float2(o[nt][i][0] + o[nt][i][1], o[nt][i][2] + o[nt][i][3])
-                             : make_float2(o[nt][i][e], o[nt][i][2 + e]);
+                    K::split ? make_float2((o[nt][i][0] + o[nt][i][1]) * kValueScale, (o[nt][i][2] + o[nt][i][3]) * kValueScale)
+                             : make_float2(o[nt][i][e] * kValueScale, o[nt][i][2 + e] * kValueScale);
             if (g == 0) {
                 ml[2 * r] = m[nt][e];
                 ml[2 * r + 1] = sum;
             }
         }
-    // whether the item begins here (the first warp knows) and ends here (the last one does)
-    if (threadIdx.x == 0) *merged_word = begin == 0 ? 2 : 1;
-    __syncthreads();
-    if (threadIdx.x == 32 * (W - 1) && ends) *abort_word = 1;
-    __syncthreads();
-    const bool starts_here = *merged_word == 2, ends_here = *abort_word != 0, whole = starts_here && ends_here;
-    const int at = 2 * blockIdx.x * W, n_rows = q.count * p.group;
-    if (threadIdx.x == 0) {
-        if (starts_here) p.items[item].x = whole ? -1 : at;
-        if (ends_here && !whole) p.items[item].y = blockIdx.x * W + W - 1;
+    bool starts_here = false, ends_here = false;
+    int at = 0;
+    const int n_rows = q.count * p.group;
+    if constexpr (cluster) {
+        __syncthreads();
+    } else {
+        // whether the item begins here (the first warp knows) and ends here (the last one does)
+        if (threadIdx.x == 0) *merged_word = begin == 0 ? 2 : 1;
+        __syncthreads();
+        if (threadIdx.x == 32 * (W - 1) && ends) *abort_word = 1;
+        __syncthreads();
+        starts_here = *merged_word == 2;
+        ends_here = *abort_word != 0;
+        at = 2 * blockIdx.x * W;
+        if (threadIdx.x == 0) {
+            if (starts_here) p.items[item].x = ends_here ? -1 : at;
+            if (ends_here && !starts_here) p.items[item].y = blockIdx.x * W + W - 1;
+        }
+        if (!(starts_here && ends_here))  // the other warps' parts are empty
+            for (int i = threadIdx.x; i < (W - 1) * K::rows; i += 32 * W)
+                *reinterpret_cast<float2 *>(p.part + ((size_t)(at + 2 * (1 + i / K::rows)) * K::rows + i % K::rows) * (D + 2) + D) =
+                    make_float2(-INFINITY, 0.0f);
     }
-    if (!whole)  // the other warps' parts are empty
-        for (int i = threadIdx.x; i < (W - 1) * K::rows; i += 32 * W)
-            *reinterpret_cast<float2 *>(p.part + ((size_t)(at + 2 * (1 + i / K::rows)) * K::rows + i % K::rows) * (D + 2) + D) =
-                make_float2(-INFINITY, 0.0f);
+    const bool whole = cluster ? ranks == 1 : starts_here && ends_here;
+    float *block_part = ml + 2 * W * K::rows;  // a cluster's: [row][D + 2]
     constexpr int per = D / 8;  // threads of a row, 8 dims each
     for (int i = threadIdx.x; i < K::rows * per; i += 32 * W) {
         const int r = i / per, d = i % per * 8;
@@ -711,70 +830,109 @@ static __global__ void __launch_bounds__(32 * kDecodeWarps, NT == 1 ? kDecodeCta
             const int token = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) - token * p.group;
             store8(static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + d, p.wide, x);
         } else {
-            float *part = p.part + ((size_t)at * K::rows + r) * (D + 2);
+            float *part = cluster ? block_part + r * (D + 2) : p.part + ((size_t)at * K::rows + r) * (D + 2);
 #pragma unroll
             for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(x[e], x[e + 1]);
             if (d == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(top, sum);
         }
     }
+    if constexpr (cluster) {
+        if (ranks == 1) return;
+        // the blocks' parts in rank order: each block finishes a share of the rows' dims
+        const cg::cluster_group group = cg::this_cluster();
+        group.sync();
+        for (int i = rank * 32 * W + threadIdx.x; i < K::rows * per; i += ranks * 32 * W) {
+            const int r = i / per, d = i % per * 8;
+            if (r0 + r >= n_rows) continue;
+            float top = -INFINITY, sum = 0.0f, x[8] = {};
+            for (int k = 0; k < ranks; k++) top = fmaxf(top, group.map_shared_rank(block_part, k)[r * (D + 2) + D]);
+#pragma unroll 4
+            for (int k = 0; k < ranks; k++) {
+                const float *part = group.map_shared_rank(block_part, k) + r * (D + 2);
+                const float2 ml2 = *reinterpret_cast<const float2 *>(part + D);
+                const float weight = ml2.y == 0.0f ? 0.0f : ml2.x == top ? 1.0f : exp2_fast(ml2.x - top);
+                sum = fmaf(weight, ml2.y, sum);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float2 v = *reinterpret_cast<const float2 *>(part + d + e);
+                    x[e] = fmaf(weight, v.x, x[e]);
+                    x[e + 1] = fmaf(weight, v.y, x[e + 1]);
+                }
+            }
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= inverse;
+            const int token = (r0 + r) / p.group, head = kvh * p.group + (r0 + r) - token * p.group;
+            store8(static_cast<T *>(p.out) + (size_t)(q.first + token) * p.out_stride + (size_t)head * D + d, p.wide, x);
+        }
+        group.sync();  // no block's shared memory goes while another reads it
+    }
 }
 
 // `Warps` warps: the parts of an item's row, in a fixed order, to a row's head. at(i) is
-// part i's D + 2 floats. Every thread of the block calls it.
+// part i's D + 2 floats. Every thread of the block calls it. What it costs is trips to
+// L2 one after the other, so a warp's parts are fetched eight at a time, the rows
+// together with their maxima and sums.
 template <int D, typename T, int Warps, typename At>
 __device__ __forceinline__ void kv4_combine(const Kv4AttnParams &p, At &&at, int parts, int row, int head)
 {
-    constexpr int per = D / 32;
+    constexpr int per = D / 32, batch = 8;
     const int lane = threadIdx.x & 31, warp = Warps == 1 ? 0 : threadIdx.x >> 5;
     float top = -INFINITY, total = 0.0f, x[per] = {};
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, at(i)[D]);
-    top = warp_max(top);
-    for (int i0 = 32 * warp; i0 < parts; i0 += 32 * Warps) {
-        float weight = 0.0f;
-        if (i0 + lane < parts) {
-            const float2 ml = *reinterpret_cast<const float2 *>(at(i0 + lane) + D);
-            weight = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2_fast(ml.x - top);
-            total = fmaf(weight, ml.y, total);
+    // a part without keys has l = 0, whatever else it holds
+    auto weigh = [&](float m, float l) { return l == 0.0f ? 0.0f : m == top ? 1.0f : exp2_fast(m - top); };
+    for (int i0 = warp; i0 < parts; i0 += batch * Warps) {
+        float2 ml[batch], v[batch][per / 2];
+#pragma unroll
+        for (int u = 0; u < batch; u++) {
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (i0 + u * Warps >= parts) continue;
+            const float *src = at(i0 + u * Warps);
+            ml[u] = *reinterpret_cast<const float2 *>(src + D);
+#pragma unroll
+            for (int e = 0; e < per / 2; e++) v[u][e] = *reinterpret_cast<const float2 *>(src + per * lane + 2 * e);
         }
-        // parts without a weight are not read
-        for (unsigned left = __ballot_sync(0xffffffffu, weight != 0.0f); left;) {
-            float v[4][per], w[4];
+        float high = top;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int i = left ? __ffs(left) - 1 : 0;
-                w[u] = __shfl_sync(0xffffffffu, weight, i);
-                if (!left) w[u] = 0.0f;
-                const float *src = at(i0 + i) + per * lane;
+        for (int u = 0; u < batch; u++) high = fmaxf(high, ml[u].x);
+        const float corr = high == top ? 1.0f : exp2_fast(top - high);
+        top = high;
+        total *= corr;
 #pragma unroll
-                for (int e = 0; e < per; e += 2) {
-                    float2 two = make_float2(0.0f, 0.0f);
-                    if (left) two = *reinterpret_cast<const float2 *>(src + e);
-                    v[u][e] = two.x, v[u][e + 1] = two.y;
-                }
-                left &= left - 1;
+        for (int e = 0; e < per; e++) x[e] *= corr;
+#pragma unroll
+        for (int u = 0; u < batch; u++) {
+            const float w = weigh(ml[u].x, ml[u].y);
+            if (w == 0.0f && ml[u].y == 0.0f) continue;
+            total = fmaf(w, ml[u].y, total);
+#pragma unroll
+            for (int e = 0; e < per; e += 2) {
+                x[e] = fmaf(w, v[u][e / 2].x, x[e]);
+                x[e + 1] = fmaf(w, v[u][e / 2].y, x[e + 1]);
             }
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int e = 0; e < per; e++) x[e] = fmaf(w[u], v[u][e], x[e]);
         }
     }
-    total = warp_sum(total);
     if (Warps > 1) {
-        __shared__ float merge[Warps][D + 1];
+        __shared__ float merge[Warps][D + 2];
 #pragma unroll
         for (int e = 0; e < per; e++) merge[warp][per * lane + e] = x[e];
-        if (lane == 0) merge[warp][D] = total;
+        if (lane == 0) {
+            merge[warp][D] = top;
+            merge[warp][D + 1] = total;
+        }
         __syncthreads();
         if (warp) return;
+#pragma unroll
+        for (int w = 1; w < Warps; w++) top = fmaxf(top, merge[w][D]);
         total = 0.0f;
 #pragma unroll
         for (int e = 0; e < per; e++) x[e] = 0.0f;
 #pragma unroll
         for (int w = 0; w < Warps; w++) {
-            total += merge[w][D];
+            const float weight = weigh(merge[w][D], merge[w][D + 1]);
+            total = fmaf(weight, merge[w][D + 1], total);
 #pragma unroll
-            for (int e = 0; e < per; e++) x[e] += merge[w][per * lane + e];
+            for (int e = 0; e < per; e++) x[e] = fmaf(weight, merge[w][per * lane + e], x[e]);
         }
     }
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
@@ -783,26 +941,25 @@ __device__ __forceinline__ void kv4_combine(const Kv4AttnParams &p, At &&at, int
     for (int e = 0; e < per; e++) dst[e] = from_float<T>(x[e] * inverse);
 }
 
-// The decode kernel's rows, [item][row of the tile]: 4 rows a block, a warp each, or,
-// where items have many parts, one row a block of 8 warps.
+// The decode kernel's rows, [item][row of the tile], a block each, of 4 warps, or 8 where
+// items have many parts (64 sequences of up to 4352 keys, decode and combine together: 42.2
+// us, with 2 warps 43.4, with 1 45.0; 4 of 8000 keys: 24.0 with 8, 26.5 by one warp that
+// fetched a part at a time).
 template <int D, typename T, int Warps>
-static __global__ void __launch_bounds__(Warps == 1 ? 128 : 32 * Warps) kv4_combine_kernel(Kv4AttnParams p, int tile_rows)
+static __global__ void __launch_bounds__(32 * Warps) kv4_combine_kernel(Kv4AttnParams p, int tile_rows)
 {
-    const int at = Warps == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, item = at / tile_rows;
+    const int at = blockIdx.x, item = at / tile_rows;
     const int r0 = item % p.tiles * tile_rows, r = r0 + at % tile_rows;
     const int kvh = item / p.tiles % p.cache.heads, s = item / p.tiles / p.cache.heads;
     pdl_wait();
     pdl_launch_dependents();
     if (s >= p.rows.sequences) return;
+    int2 where = p.items[item];
     const Kv4Sequence q = kv4_sequence(p.rows, s);
     if (!q.ok || q.count * p.group > p.most || r >= q.count * p.group) return;
     const int token = r / p.group, head = kvh * p.group + r - token * p.group;
-    int2 where = make_int2(0, -1);  // no keys: no parts
-    if (q.length > 0) {
-        where.x = p.items[item].x;
-        if (where.x < 0) return;
-        where.y = p.items[item].y;
-    }
+    if (q.length <= 0) where = make_int2(0, -1);  // no keys: no parts
+    else if (where.x < 0) return;
     // the first part, then the first of each warp up to the last
     const float *part = p.part + (size_t)(r - r0) * (D + 2);
     const int first_warp = where.x >> 1;

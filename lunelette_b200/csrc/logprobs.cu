@@ -19,20 +19,7 @@ template <typename T, int THREADS> cudaError_t launch_clusters(LogprobParams p, 
     constexpr int smem = (int)sizeof(LogprobShared<THREADS>);
     const cudaError_t e = opt_in<logprobs_kernel<T, THREADS>>(smem, true);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((size_t)p.rows * p.parts));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    return launch_cluster(kernel, dim3((unsigned)((size_t)p.rows * p.parts)), dim3(THREADS), smem, p.parts, stream, p);
 }
 
 // CTAs of a row: up to 16, while there are fewer than about one an SM and each
