@@ -29,13 +29,13 @@
 // bits of one FP16 are taken (q exact after a power-of-two scaling but for what lies
 // 2^-17 below the row's largest; a weight off by 2^-12 of itself, under the rounding of the
 // output), 8 rows an MMA.
-// A code needs no arithmetic to become FP16: four bits alone in a half's lowest eight are a
-// subnormal, c * 2^-24 or c * 2^-20, which one AND leaves.
-//   S = K Q^T     A: 16 keys x 16 dims of codes as they are; q is times 2^14 or 2^10 to
-//                 match, -8 sum q is what a group's sum starts from, and it is scaled by d in FP32
-//                 after its two MMAs.
-//   O^T = V^T P^T A: 16 dims x 16 keys of d * (c - 8) * 2^-9, one fused multiply-add from
-//                 the code, whose exact result FP16 holds while 2^-8 <= |d| < 2; a page with
+//   S = K Q^T     A: 16 keys x 16 dims of c - 8 (an AND and a subtraction); a group's sum, in FP32, is
+//                 scaled by d after its two MMAs. Codes as they are, with -8 sum q to start a sum
+//                 from, take as long and lose six times as much: the tensor core cuts sums to FP32
+//                 towards zero, and those are larger.
+//   O^T = V^T P^T A: 16 dims x 16 keys of d * (c - 8) * 2^-9. Four bits alone in a half's lowest eight
+//                 are a subnormal, c * 2^-24 or c * 2^-20, that one AND leaves; one fused multiply-add
+//                 follows, whose exact result FP16 holds while 2^-8 <= |d| < 2; a page with
 //                 another d takes two more steps a code. B: the weights, moved from S's layout by
 //                 movmatrix.
 #pragma once
@@ -402,7 +402,6 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
         const int n_rows = q.count * p.group, units = (q.length + 16 * KT - 1) / (16 * KT);
         // q as B: column g of n tile nt belongs to row (split: 4 nt + g / 2, part g % 2; else 8 nt + g)
         uint32_t qb[NT][D / 16][2];
-        float minus8[NT][G][2];  // -8 sum q of a group, as the products count it, of columns 2 t and 2 t + 1
         float back[NT][RP];      // what a score is multiplied with, of the lane's rows 4 nt + t or 8 nt + 2 t + (0, 1)
         int limit[NT][RP];   // those rows' last visible position
 #pragma unroll
@@ -431,27 +430,14 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                 for (int hw = 0; hw < 2; hw++)
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
-                        uint32_t hi, lo;  // low nibbles are 2^-4 of high ones
-                        const float up = b ? 0x1p10f * f : 0x1p14f * f;
-                        split_half2(x[j][2 * hw + b] * up, x[j][2 * hw + b + 4] * up, hi, lo);
+                        uint32_t hi, lo;
+                        split_half2(x[j][2 * hw + b] * f, x[j][2 * hw + b + 4] * f, hi, lo);
                         qb[nt][2 * j + hw][b] = K::split && (g & 1) ? lo : hi;
                     }
 #pragma unroll
-            for (int j = 0; j < G; j++) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int hw = 0; hw < 2; hw++)
-                    sum += (low_half(qb[nt][2 * j + hw][0]) + high_half(qb[nt][2 * j + hw][0])) * -0x1p-21f +
-                           (low_half(qb[nt][2 * j + hw][1]) + high_half(qb[nt][2 * j + hw][1])) * -0x1p-17f;
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                minus8[nt][j][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-                minus8[nt][j][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-            }
-#pragma unroll
             for (int e = 0; e < RP; e++) {
                 // the row's factors sit in the lanes of its (first) column
-                back[nt][e] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + e)) * (p.scale2 * 0x1p10f);
+                back[nt][e] = __shfl_sync(0xffffffffu, undo, 4 * (2 * t + e)) * p.scale2;
                 const int row = r0 + (K::split ? 4 * nt + t : 8 * nt + 2 * t + e);
                 limit[nt][e] = row < n_rows ? q.length - q.count + row / p.group : -1;
                 m[nt][e] = -INFINITY;
@@ -498,14 +484,14 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                 }
 #pragma unroll
                 for (int j = 0; j < G; j++) {
-                    const uint32_t a0[4] = {kv4_code(ka[j]), kv4_code(kb[j]), kv4_code16(ka[j]), kv4_code16(kb[j])};
-                    const uint32_t a1[4] = {kv4_code(ka[j] >> 8), kv4_code(kb[j] >> 8), kv4_code16(ka[j] >> 8),
-                                            kv4_code16(kb[j] >> 8)};
+                    const uint32_t a0[4] = {kv4_low(ka[j]), kv4_low(kb[j]), kv4_high(ka[j]), kv4_high(kb[j])};
+                    const uint32_t a1[4] = {kv4_low(ka[j] >> 8), kv4_low(kb[j] >> 8), kv4_high(ka[j] >> 8),
+                                            kv4_high(kb[j] >> 8)};
                     const float d0 = j & 1 ? high_half(da[j >> 1]) : low_half(da[j >> 1]);
                     const float d1 = j & 1 ? high_half(db[j >> 1]) : low_half(db[j >> 1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float c[4] = {minus8[nt][j][0], minus8[nt][j][1], minus8[nt][j][0], minus8[nt][j][1]};
+                        float c[4] = {};
                         mma_16816(c, a0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
                         mma_16816(c, a1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
                         acc[nt][0] = fmaf(d0, c[0], acc[nt][0]);

@@ -22,6 +22,9 @@
 // running maximum is kept until a tile raises it by more than 2^8 (a raise waits for
 // P V and rescales O, up to 2000 cycles; with 2^4 half the tiles had one), so a weight is at
 // most 2^15, and its parts end at 2^-32 of the largest.
+// The tensor core cuts every sum to FP32 towards zero, so hundreds of them in a row into O lose
+// more than FP32 should (5.8e-6 of the outputs' norm at 4352 keys). For FP32 rows the softmax
+// takes O out every 8 tiles and sums those in shared memory, rounded to nearest.
 //
 // A code pair leaves the conversion as dims (n, n + 4) of a word, so each 8 dims lie
 // in the order 0 4 1 5 2 6 3 7 in K and V and, to match, in Q and O.
@@ -36,6 +39,7 @@ namespace lun {
 
 constexpr int kBlockRows = 128, kBlockThreads = 448, kBlockStages = 6;
 constexpr float kBlockShift = 7.0f, kBlockRaise = 8.0f;
+constexpr int kBlockDrain = 8;
 
 template <int D> struct Kv4BlockLayout {
     static constexpr int half = Kv4Layout<D>::block / 2;
@@ -289,11 +293,12 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                 const uint32_t sd = tmem + s_col + 128u * (uint32_t)b;
                 const uint64_t k = k_desc + (uint32_t)b * (2 * B::tile >> 4);
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks++)
+                for (int part = parts - 1; part >= 0; part--)  // the small sums first
 #pragma unroll
-                    for (int part = 0; part < parts; part++)
+                    for (int ks = 0; ks < D / 16; ks++)
                         tc_mma_f16_tmem_a(sd, tmem + q_col + 64u * part + 8u * ks,
-                                          k + (((ks >> 2) * 16384 + (ks & 3) * 32) >> 4), idesc, (ks | part) != 0);
+                                          k + (((ks >> 2) * 16384 + (ks & 3) * 32) >> 4), idesc,
+                                          ks != 0 || part != parts - 1);
                 tc_commit(&k_free[b]);
                 tc_commit(&s_full[b]);
             }
@@ -316,7 +321,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
 #pragma unroll
                     for (int part = 0; part < parts; part++)
                         tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, v + (ks * 2048 >> 4), idesc_o,
-                                          ks || part || j > 0);
+                                          ks || part || (parts == 2 ? j % kBlockDrain != 0 : j > 0));
                 tc_commit(&v_free[b]);
                 tc_commit(&o_done[b]);
             }
@@ -469,6 +474,9 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         }
         const int all_see = first_position + t0;  // every live row sees keys up to here
         float m = -INFINITY, l = 0.0f;
+        // FP32: what O held every kBlockDrain tiles, and what has scaled it since; where q's row was
+        float4 *drained = reinterpret_cast<float4 *>(base + B::q_rows + row * B::q_stride);
+        float since = 1.0f;
         bool ok = true;
         for (int j = 0; j < tiles; j++) {
             if (!(ok = kv4_warp_wait(&s_full[j >> 1 & 1], (j >> 2) & 1, abort_word))) break;
@@ -497,7 +505,26 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             const bool raise = m != -INFINITY && (mx - m) * back > kBlockRaise;
             const float corr = raise ? exp2_fast((m - mx) * back) : 1.0f;
             if (m == -INFINITY || raise) m = mx;
-            if (__any_sync(0xffffffffu, raise)) {
+            if (parts == 2 && j > 0 && j % kBlockDrain == 0) {
+                // P V of the tile before has landed, and P V of this one starts from zero
+                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(lane_base + o_col + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 sum = j == kBlockDrain ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : drained[(c + i) / 4];
+                        sum.x = fmaf(sum.x, since, __uint_as_float(o[i]));
+                        sum.y = fmaf(sum.y, since, __uint_as_float(o[i + 1]));
+                        sum.z = fmaf(sum.z, since, __uint_as_float(o[i + 2]));
+                        sum.w = fmaf(sum.w, since, __uint_as_float(o[i + 3]));
+                        drained[(c + i) / 4] = sum;
+                    }
+                }
+                since = corr;
+            } else if (__any_sync(0xffffffffu, raise)) {
                 // O's row *= corr once P V of the tile before has landed
                 if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
                 tc_fence_after();
@@ -509,6 +536,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                     for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
                     tmem_st32(lane_base + o_col + c, o);
                 }
+                since *= corr;
             }
             l *= corr;
             const float zero = m == -INFINITY ? 0.0f : -m;
@@ -567,6 +595,16 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                     for (int i = 0; i < 32; i++) o[i] = 0u;
                 }
                 if (!live) continue;
+                if (parts == 2 && tiles > kBlockDrain) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 sum = drained[(c + i) / 4];
+                        o[i] = __float_as_uint(fmaf(sum.x, since, __uint_as_float(o[i])));
+                        o[i + 1] = __float_as_uint(fmaf(sum.y, since, __uint_as_float(o[i + 1])));
+                        o[i + 2] = __float_as_uint(fmaf(sum.z, since, __uint_as_float(o[i + 2])));
+                        o[i + 3] = __float_as_uint(fmaf(sum.w, since, __uint_as_float(o[i + 3])));
+                    }
+                }
                 const bool nan = limit >= poison[c / kKv4Group];
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
