@@ -227,7 +227,8 @@ size_t lunelette_cuda_kv4_bytes(size_t layers, size_t pages, size_t kv_heads, si
  * The functions that take a device word `status` (or NULL) OR 1 into it when a
  * sequence breaks these bounds or its offsets descend (its rows are skipped and
  * left as they are), and 2 when a page lies outside the pool (its positions are
- * skipped). Sequences may be empty, and a row before position 0 (n > length)
+ * skipped); attention ORs 4 when a copy or a tensor-core step has not come back
+ * for a second, and its outputs are not valid then. Sequences may be empty, and a row before position 0 (n > length)
  * has no position: nothing is stored or read for it. Sequences of one call must
  * not append to the same page. */
 typedef struct lunelette_cuda_rows {
