@@ -360,7 +360,9 @@ def attention_check(torch, c, held, name, group, scale, seed, first=None):
     q64 = q.double().cpu().numpy().reshape(c.rows, query, c.dim)
     for s, (n, length) in enumerate(zip(c.counts, c.lengths)):
         r = slice(int(c.offsets[s]), int(c.offsets[s]) + n)
-        want, *size = ref.attention(q64[r], held[s][0], held[s][1], scale, length - n)
+        want, *size = (np.concatenate(parts, 1) for parts in zip(*(
+            ref.attention(q64[r, h * group:(h + 1) * group], held[s][0][:, h:h + 1].astype(np.float64),
+                          held[s][1][:, h:h + 1].astype(np.float64), scale, length - n) for h in range(c.heads))))
         check_rows(torch, name, got[r], want, *size)
     assert (got[int(c.offsets[-1]):] == 7.0).all()
     assert c.status.item() == 0
@@ -409,6 +411,11 @@ ATTENTION = [  # type, dim, kv heads, group, counts, lengths, unused rows
     ("bf16", 64, 1, 40, [5, 1], [70, 200], 0),
     ("f32", 64, 1, 1, [300], [300], 0),
     ("f32", 128, 1, 2, [100, 1, 40], [60, 0, 41], 0),        # rows before position 0, an empty cache
+    ("f16", 64, 1, 130, [1, 2], [70, 65], 0),                # a group beyond a tile's rows
+    ("bf16", 64, 256, 1, [1, 0, 1], [20, 0, 66], 1),         # as many KV heads as there may be
+    ("f32", 128, 2, 2, [1] * 150, [1 + 37 * i % 200 for i in range(150)], 0),
+    ("f16", 64, 2, 1, ([1] * 9 + [0]) * 40, ([5, 64, 0, 131, 17, 65, 1, 30, 128, 9] * 40), 3),  # 400 sequences
+    ("f32", 64, 1, 2, [1] * 299 + [30], [1 + i % 90 for i in range(299)] + [50], 0),
 ]
 
 
@@ -417,6 +424,33 @@ def test_attention_matches_definition(torch, name, dim, heads, group, counts, le
     c = Cache(torch, counts, lengths, heads, dim, pad=pad, seed=len(counts))
     held = c.fill(np.random.default_rng(sum(lengths) + dim))
     attention_check(torch, c, held, name, group, dim ** -0.5, seed=dim + sum(counts))
+
+
+def over_shared_pages(torch, counts, lengths, heads, dim, pages, seed):
+    """A cache whose sequences hold the same few pages again and again; and what they read."""
+    c = Cache(torch, [0], [64 * pages], heads, dim, seed=seed, spare=0)
+    (k, v), = c.fill(np.random.default_rng(seed))
+    by_page = np.argsort(c.table[0, :pages])  # the sequence's page that lies at a place of the pool
+    c.counts, c.lengths = list(counts), list(lengths)
+    c.stride = -(-max(lengths) // 64)
+    c.table = np.random.default_rng(seed + 1).integers(0, pages, (len(counts), c.stride)).astype(np.int32)
+    c.offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    c.rows, c.max_count, c.max_length = int(c.offsets[-1]), max(counts), max(lengths)
+    c.d_offsets, c.d_table = torch.from_numpy(c.offsets).cuda(), torch.from_numpy(c.table).cuda()
+    c.d_lengths = torch.tensor(c.lengths, dtype=torch.int32, device="cuda")
+    k, v = (x.reshape(pages, 64, heads, dim).astype(np.float16) for x in (k, v))  # exact
+    return c, [[x[by_page[c.table[s, :-(-n // 64)]]].reshape(-1, heads, dim)[:n] for x in (k, v)]
+               for s, n in enumerate(lengths)]
+
+
+@pytest.mark.parametrize("name,dim,heads,group,counts,lengths", [
+    ("f32", 64, 16, 5, [1, 1], [160000, 150001]),                        # more than 64 pages a warp
+    ("f16", 128, 2, 1, [1] * 3, [200000, 70, 130001]),
+    ("f16", 64, 32, 1, [20] * 5, [6000, 5999, 4097, 5000, 4160]),        # more than 64 pages a block
+    ("f32", 128, 4, 4, [32] * 10, [5000] * 10)])
+def test_attention_over_pages_held_many_times(torch, name, dim, heads, group, counts, lengths):
+    c, held = over_shared_pages(torch, counts, lengths, heads, dim, 8, seed=40)
+    attention_check(torch, c, held, name, group, dim ** -0.5, seed=41)
 
 
 def test_attention_ignores_stale_slots_and_other_pages(torch):
@@ -647,19 +681,22 @@ def test_side_stream_and_captured_graph_follow_later_lengths(torch):
     assert c.status.item() == 0
 
 
-def test_two_graphs_with_a_workspace_each_overlap(torch):
+@pytest.mark.parametrize("heads,two", [(1, [([1], [4000]), ([1, 1], [3000, 2000])]),
+                                       (2, [([1], [9000]), ([1] * 30, [300 + 41 * i for i in range(30)])]),
+                                       (2, [([150], [2000]), ([40, 1, 3, 70, 1, 1], [900, 700, 64, 1000, 5, 333])])])
+def test_two_graphs_with_a_workspace_each_overlap(torch, heads, two):
     """Two captured attention calls on two streams at once, each with its workspace."""
-    calls = []
-    for seed, (counts, lengths) in enumerate([([1], [4000]), ([1, 1], [3000, 2000])]):
-        c = Cache(torch, counts, lengths, 1, 128, seed=seed)
+    calls, group = [], 4
+    for seed, (counts, lengths) in enumerate(two):
+        c = Cache(torch, counts, lengths, heads, 128, seed=seed)
         held = c.fill(np.random.default_rng(seed))
-        q, out = attention_check(torch, c, held, "f32", 4, 0.09, seed=seed)
-        ws, got, stream = c.workspace(4), torch.zeros_like(out), torch.cuda.Stream()
+        q, out = attention_check(torch, c, held, "f32", group, 0.09, seed=seed)
+        ws, got, stream = c.workspace(group * heads), torch.zeros_like(out), torch.cuda.Stream()
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         with torch.cuda.graph(graph, stream=stream):
             assert L.library().lunelette_cuda_kv4_attention(
-                c.kv4(), c.layer, c.descriptor(), L.FLOAT32, q.data_ptr(), q.stride(0), 4, 0.09, got.data_ptr(),
+                c.kv4(), c.layer, c.descriptor(), L.FLOAT32, q.data_ptr(), q.stride(0), group * heads, 0.09, got.data_ptr(),
                 got.stride(0), ws.data_ptr(), ws.numel(), None, c.stream()) == 0
         calls.append((c, q, out, ws, got, stream, graph))
     torch.cuda.synchronize()
