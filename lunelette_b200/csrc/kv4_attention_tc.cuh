@@ -24,7 +24,12 @@
 // most 2^15, and its parts end at 2^-32 of the largest.
 // The tensor core cuts every sum to FP32 towards zero, so hundreds of them in a row into O lose
 // more than FP32 should (5.8e-6 of the outputs' norm at 4352 keys). For FP32 rows the softmax
-// takes O out every 8 tiles and sums those in shared memory, rounded to nearest.
+// takes O out every 8 tiles and sums those in shared memory, rounded to nearest (1.65e-6, and
+// 49.1 -> 54.2 us for 256 tokens).
+//
+// 256 FP32 tokens at 4352 keys, 8 KV heads of 4 query heads, with the combine: 54 us, 330 TFLOP/s
+// of the definition's products and twice that issued; a tile takes 1300 to 1750 cycles, bound by
+// the softmax warps' arithmetic.
 //
 // A code pair leaves the conversion as dims (n, n + 4) of a word, so each 8 dims lie
 // in the order 0 4 1 5 2 6 3 7 in K and V and, to match, in Q and O.

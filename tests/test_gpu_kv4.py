@@ -415,6 +415,7 @@ ATTENTION = [  # type, dim, kv heads, group, counts, lengths, unused rows
     ("bf16", 64, 256, 1, [1, 0, 1], [20, 0, 66], 1),         # as many KV heads as there may be
     ("f32", 128, 2, 2, [1] * 150, [1 + 37 * i % 200 for i in range(150)], 0),
     ("f16", 64, 2, 1, ([1] * 9 + [0]) * 40, ([5, 64, 0, 131, 17, 65, 1, 30, 128, 9] * 40), 3),  # 400 sequences
+    ("f32", 64, 2, 1, [1] * 200, [0] * 200, 0),              # nothing anywhere
     ("f32", 64, 1, 2, [1] * 299 + [30], [1 + i % 90 for i in range(299)] + [50], 0),
 ]
 
