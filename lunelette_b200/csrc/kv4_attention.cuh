@@ -27,10 +27,10 @@
 // decode step has 1 to 16 query rows a KV head, so a tcgen05 tile of 128 rows would be
 // mostly padding, while here the rows sit in the n = 8 side. FP32 rows of q and
 // weights of the softmax enter as FP16 hi + lo parts in neighbouring columns
-// (22 bits together), so one MMA serves 4 rows at FP32 grade; of 16-bit rows the 11
-// bits of one FP16 are taken (q exact after a power-of-two scaling but for what lies
-// 2^-17 below the row's largest; a weight off by 2^-12 of itself, under the rounding of the
-// output), 8 rows an MMA.
+// (22 bits together), so one MMA serves 4 rows at FP32 grade. Of 16-bit rows q is one FP16
+// (exact after a power-of-two scaling but for what lies below 2^-24 of the row's largest), 8
+// rows an MMA; their weights are two FP16 all the same, in two MMAs (with one, off by 2^-12,
+// FP16 outputs lost a fifth more than their own rounding does).
 //   S = K Q^T     A: 16 keys x 16 dims of c - 8 (an AND and a subtraction); a group's sum, in FP32, is
 //                 scaled by d after its two MMAs. Codes as they are, with -8 sum q to start a sum
 //                 from, take as long and lose six times as much: the tensor core cuts sums to FP32
@@ -585,7 +585,7 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                 }
             }
             const float shift = small ? kWeightShift : kWeightShift - kValueShift, count = small ? 1.0f : kValueScale;
-            uint32_t pb[KT][NT][2];
+            uint32_t pb[KT][NT][2], pl[KT][NT][2];  // pl: 16-bit rows' lo parts
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 // the maximum moves seldom once a few pages are in: the warp agrees on whether one does
@@ -636,6 +636,8 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                             two = __halves2half2(h, __float2half_rn(w[0] - __half2float(h)));
                         } else {
                             two = __floats2half2_rn(w[0], w[1]);
+                            const __half2 rest = __floats2half2_rn(w[0] - __low2float(two), w[1] - __high2float(two));
+                            pl[tile][nt][k8] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&rest));
                         }
                         pb[tile][nt][k8] = movmatrix_trans(*reinterpret_cast<const uint32_t *>(&two));
                     }
@@ -686,8 +688,11 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                                     a[3] = kv4_times(kv4_high(y1), d2[1]);
                                 }
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++)
-                                    mma_16816(o[nt][4 * w + 2 * half + two], a, pb[tile][nt][0], pb[tile][nt][1]);
+                                for (int nt = 0; nt < NT; nt++) {
+                                    float (&sum)[4] = o[nt][4 * w + 2 * half + two];
+                                    if constexpr (!K::split) mma_16816(sum, a, pl[tile][nt][0], pl[tile][nt][1]);
+                                    mma_16816(sum, a, pb[tile][nt][0], pb[tile][nt][1]);
+                                }
                             }
                         }
                 }

@@ -17,8 +17,8 @@
 //               row's 64 scores from tensor memory, causal mask, online softmax,
 //               weights over the scores as the A operand of P V; at the end O / l or
 //               the split's part.
-// FP32 rows go in as FP16 hi + lo parts (two MMAs a product, 22 bits; the cache's
-// side is exact in one part), 16-bit rows as one. Weights are times 2^7, and the
+// FP32 rows of q go in as FP16 hi + lo parts (two MMAs a product, 22 bits; the cache's
+// side is exact in one part), 16-bit rows as one, and the weights of either in two. Weights are times 2^7, and the
 // running maximum is kept until a tile raises it by more than 2^8 (a raise waits for
 // P V and rescales O, up to 2000 cycles; with 2^4 half the tiles had one), so a weight is at
 // most 2^15, and its parts end at 2^-32 of the largest.
@@ -324,7 +324,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
 #pragma unroll
                 for (int ks = 0; ks < kPage / 16; ks++)
 #pragma unroll
-                    for (int part = 0; part < parts; part++)
+                    for (int part = 0; part < 2; part++)
                         tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, v + (ks * 2048 >> 4), idesc_o,
                                           ks || part || (parts == 2 ? j % kBlockDrain != 0 : j > 0));
                 tc_commit(&v_free[b]);
@@ -556,23 +556,19 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                 b = exp2_fast(b);
                 const uint64_t ab = pack2(a, b);
                 sum = add_f32x2(sum, ab);
-                if (parts == 2) {
-                    // hi: the 11 leading bits, lo: the rest
-                    const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u);
-                    const float hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
-                    float la, lb;
-                    unpack2(add_f32x2(ab, pack2(-ha, -hb)), la, lb);
-                    ph[i] = half2_bits(ha, hb);
-                    pl[i] = half2_bits(la, lb);
-                } else {
-                    ph[i] = half2_bits(a, b);
-                }
+                // hi: the 11 leading bits, lo: the rest
+                const float ha = __uint_as_float(__float_as_uint(a) & 0xffffe000u);
+                const float hb = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+                float la, lb;
+                unpack2(add_f32x2(ab, pack2(-ha, -hb)), la, lb);
+                ph[i] = half2_bits(ha, hb);
+                pl[i] = half2_bits(la, lb);
             }
             float sum0, sum1;
             unpack2(sum, sum0, sum1);
             l += sum0 + sum1;
             tmem_st32(lane_base + sb, ph);
-            if (parts == 2) tmem_st32(lane_base + sb + 32u, pl);
+            tmem_st32(lane_base + sb + 32u, pl);
             tc_fence_before();
             // not more than two tiles ahead of P V: a barrier's parity tells only two
             // phases in a row apart, here of p_ready (whose last one the issuer has then seen) and of
