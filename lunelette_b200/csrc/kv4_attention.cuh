@@ -40,6 +40,13 @@
 //                 follows, whose exact result FP16 holds while 2^-8 <= |d| < 2; a page with
 //                 another d takes two more steps a code. B: the weights, moved from S's layout by
 //                 movmatrix.
+// The tensor core cuts what it adds up towards zero: over values of one sign, about 1.9e-7 of the
+// sum so far each time, so that 443 pages in a row (64 FP32 sequences of 131072 keys) lost 1.7e-4.
+// So the list's warps take O out every 4 pages (16-bit rows, which add up two products a step, every
+// 12) and add those sums up to nearest: 1.4e-6 there, 0.9e-6 over 68 pages. Four FP32 sequences of
+// 131072 keys take 126 us for 122, four BF16 ones with 8 rows 151 for 146. L2's own additions
+// (red.add), which nothing waits for, take 132 and 156. A cluster's warps add up 4 units of 16
+// keys at most.
 #pragma once
 #include "async.cuh"
 #include "attention.cuh"
@@ -110,6 +117,7 @@ template <int D, typename T, int NT, int W> struct Kv4Decode {
     static constexpr int rows = 4 * NT * lane_rows;  // query rows of a tile
     static constexpr int keys = W > kListWarps ? 16 : 64;  // of a unit
     static constexpr int slots = W > kListWarps ? kClusterSlots : kListSlots;
+    static constexpr int drain = split ? 4 : 12;  // pages that the list sums up on the tensor cores
     static constexpr int codes = keys * D / 2;
     static constexpr int half = codes + keys * 2 * (D / 32);  // K or V of a unit, laid out as in a page
     static constexpr int ring = W * slots * half;
@@ -378,6 +386,7 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
     };
     float m[NT][RP], l[NT][RP], o[NT][MT][4];
+    float since[NT][RP];  // the list: what has scaled o since it was taken out last
     int item = 0, begin = 0, r0 = 0, kvh = 0;
     Kv4Sequence q = {0, 0, 0, false};
     if (cluster) {  // a warp without units has a part too
@@ -444,12 +453,50 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                 limit[nt][e] = row < n_rows ? q.length - q.count + row / p.group : -1;
                 m[nt][e] = -INFINITY;
                 l[nt][e] = 0.0f;
+                since[nt][e] = 1.0f;
             }
 #pragma unroll
             for (int j = 0; j < MT; j++) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.0f;
         }
         const int all_see = q.length - q.count + r0 / p.group;  // every row of the tile sees keys up to here
+        // The list takes o out every K::drain pages, into the place of the part that it would leave, a lane
+        // its own values (an FP32 row's two columns as one): sum * since + o.
+        float4 *sums = nullptr;
+        if constexpr (!cluster)
+            sums = reinterpret_cast<float4 *>(p.part + (size_t)(2 * me + (first_item ? 0 : 1)) * K::rows * (D + 2)) + lane;
+        auto drain = [&](bool has, bool last) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < MT; j += K::split ? 2 : 1) {
+                    float (&a)[4] = o[nt][j], (&b)[4] = o[nt][K::split ? j + 1 : j];
+                    float4 *at = sums + 32 * (nt * MT + j) / (K::split ? 2 : 1);
+                    float4 v = K::split ? make_float4(a[0] + a[1], a[2] + a[3], b[0] + b[1], b[2] + b[3])
+                                        : make_float4(a[0], a[1], a[2], a[3]);
+                    if (has) {
+                        const float4 before = *at;
+                        const float s0 = since[nt][0], s1 = K::split ? s0 : since[nt][RP - 1];
+                        v.x = fmaf(before.x, s0, v.x), v.y = fmaf(before.y, s1, v.y);
+                        v.z = fmaf(before.z, s0, v.z), v.w = fmaf(before.w, s1, v.w);
+                    }
+                    if (!last) {
+                        *at = v;
+                        v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+                    if constexpr (K::split) {
+                        a[0] = v.x, a[2] = v.y, b[0] = v.z, b[2] = v.w;
+                        a[1] = a[3] = b[1] = b[3] = 0.0f;
+                    } else {
+                        a[0] = v.x, a[1] = v.y, a[2] = v.z, a[3] = v.w;
+                    }
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < RP; e++) since[nt][e] = 1.0f;
+        };
         do {
+            if (!cluster && unit != begin && (unit - begin) % K::drain == 0) drain(unit - begin > K::drain, false);
             if ((i & 31) == 0 && i + 32 < n) {  // the other set of units, long before it is asked for
                 s = __shfl_sync(0xffffffffu, s, 31);
                 base = __shfl_sync(0xffffffffu, base, 31);
@@ -611,6 +658,7 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
                         corr[e] = mx == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - mx);
                         m[nt][e] = mx;
                         l[nt][e] *= corr[e];
+                        if (!cluster) since[nt][e] *= corr[e];
                     }
 #pragma unroll
                     for (int j = 0; j < MT; j++)
@@ -702,6 +750,10 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
             next(2 * i + 1);
         } while (unit++, ++i < n && item_at(i) == item);
         ends = unit == units;
+        if (!cluster && ok && unit - begin > K::drain) {
+            drain(true, true);
+            __syncwarp();  // the part's place is written by other lanes from here on
+        }
         if (ok && !merged) {
             // the item's end in this warp: the output where all of it was, else a part
             const bool whole = begin == 0 && ends;

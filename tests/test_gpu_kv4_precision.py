@@ -67,3 +67,71 @@ def test_16_bit_rows_are_rounded_once(torch, name, dim, heads, group, counts, le
         if n:
             check_rounded_once(torch, name, got[r], *ref.attention(q64[r], *held[s], dim ** -0.5, length - n))
     assert c.status.item() == 0
+
+
+def walk(torch, name, dim, heads, group, counts, pages, mean, seed):  # noqa: F811
+    """Sequences of `pages` whole pages each, drawn from eight that hold values around `mean`. Returns
+    outputs, their definition in 64 bits and sum p |v|, [rows, heads, group, dim]."""
+    rng = np.random.default_rng(seed)
+    held, few = [], 8
+    c = Cache(torch, [0], [64 * few], heads, dim, seed=seed, spare=0, layers=1, layer=0)
+    for kind in (0, 1):
+        x = rng.standard_normal((64 * few, heads, dim)) * (1.0 if kind == 0 else 0.25) + (0.0 if kind == 0 else mean)
+        codes, d = ref.quantise(x)
+        for p in range(64 * few):
+            ref.store(c.host[0], dim, p // 64, p % 64, codes[p], d[p], kind)
+        held.append(torch.from_numpy(ref.dequantise(codes, d).reshape(few, 64, heads, dim)).cuda())
+    c.pool.copy_(torch.from_numpy(c.host.reshape(-1)))
+    c.counts, c.lengths, c.stride = list(counts), [64 * pages] * len(counts), pages
+    c.table = rng.integers(0, few, (len(counts), pages)).astype(np.int32)
+    c.offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    c.rows, c.max_count, c.max_length = int(c.offsets[-1]), max(counts), 64 * pages
+    c.d_offsets, c.d_table = torch.from_numpy(c.offsets).cuda(), torch.from_numpy(c.table).cuda()
+    c.d_lengths = torch.tensor(c.lengths, dtype=torch.int32, device="cuda")
+    query, scale = heads * group, dim ** -0.5
+    q = tensor(torch, name, rng.standard_normal((c.rows, query * dim)))
+    out = torch.zeros_like(q)
+    c.attend(name, q, query, scale, out)
+    assert c.status.item() == 0
+    k, v = held
+    want, size = (torch.zeros((c.rows, heads, group, dim), dtype=torch.float64, device="cuda") for _ in range(2))
+    for s, n in enumerate(counts):
+        rows = q[c.offsets[s]:c.offsets[s] + n].double().reshape(n, heads, group, dim)
+        times = torch.from_numpy(np.bincount(c.table[s, :-1], minlength=few).astype(np.float64)).cuda()
+        last = int(c.table[s, -1])
+        scores = scale * torch.einsum("nhgd,pkhd->nhgpk", rows, k)
+        w = torch.exp(scores - scores.amax((-2, -1), keepdim=True))
+        seen = torch.arange(64, device="cuda")[None] <= 64 - n + torch.arange(n, device="cuda")[:, None]
+        w = torch.cat([w * times[:, None], w[..., last:last + 1, :] * seen[:, None, None, None]], -2)
+        w = w / w.sum((-2, -1), keepdim=True)
+        values = torch.cat([v, v[last:last + 1]])
+        at = slice(int(c.offsets[s]), int(c.offsets[s]) + n)
+        want[at] = torch.einsum("nhgpk,pkhd->nhgd", w, values)
+        size[at] = torch.einsum("nhgpk,pkhd->nhgd", w, values.abs())
+    return out.double().reshape(want.shape), want, size
+
+
+WALKS = [  # type, dim, kv heads, group, counts, pages of a sequence
+    ("f32", 128, 8, 4, [1] * 300, 68),       # 300 sessions of 4352 keys: 69 pages a warp
+    ("f32", 128, 8, 4, [1] * 64, 2048),      # 443 pages a warp
+    ("f32", 64, 2, 4, [2] * 5, 2048),        # two tiles of rows a warp
+    ("f32", 64, 256, 1, [1] * 40, 40),       # shares of several whole items
+    ("bf16", 128, 8, 8, [1] * 64, 2048),
+    ("f16", 128, 8, 4, [1] * 64, 2048),
+    ("f16", 64, 16, 16, [1] * 30, 1500)]
+
+
+@pytest.mark.parametrize("name,dim,heads,group,counts,pages", WALKS)
+@pytest.mark.parametrize("mean", [2.0, 0.0])
+def test_long_walks_keep_their_accuracy(torch, name, dim, heads, group, counts, pages, mean):  # noqa: F811
+    got, want, size = walk(torch, name, dim, heads, group, counts, pages, mean, seed=pages + heads)
+    # scores here are sums of 128 products of size one, 2^-21 of which moves a weight by under 2^-18; it moves
+    # an output only as far as its values differ, 1/8 of their mean here and all of them around zero
+    e = cut(name) + 2.0 ** -20 + 2.0 ** -18 * (0.125 if mean else 1.0)
+    error = (got - want).abs()
+    if name == "f32":
+        assert (error.norm() / size.norm()).item() <= e
+    else:
+        half = half_step(torch, name)
+        bound = half * want.abs() + (1 + half) * size * e + (2.0 ** -25 if name == "f16" else 0.0)
+        assert (error / bound).max().item() <= 1.0
