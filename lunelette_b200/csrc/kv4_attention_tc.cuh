@@ -22,10 +22,12 @@
 // running maximum is kept until a tile raises it by more than 2^8 (a raise waits for
 // P V and rescales O, up to 2000 cycles; with 2^4 half the tiles had one), so a weight is at
 // most 2^15, and its parts end at 2^-32 of the largest.
-// The tensor core cuts every sum to FP32 towards zero, so hundreds of them in a row into O lose
-// more than FP32 should (5.8e-6 of the outputs' norm at 4352 keys). For FP32 rows the softmax
-// takes O out every 8 tiles and sums those in shared memory, rounded to nearest (1.65e-6, and
-// 49.1 -> 54.2 us for 256 tokens).
+// The tensor core cuts what it adds up towards zero, over values of one sign about 1.7e-7 of the sum
+// so far each time. So the softmax takes O out every 4 tiles, 32 products (16-bit rows: every 8,
+// their own rounding is far larger), and sums those in shared memory, rounded to nearest, after the
+// tile's weights, when P V of the tile before has mostly landed: 2.7e-6 over 500 or 2048 tiles of one
+// sign, 0.9e-6 around zero. l is summed up with what its additions round off: 2048 tiles that
+// repeat a few sums lost 5e-6 without.
 //
 // 256 FP32 tokens at 4352 keys, 8 KV heads of 4 query heads, with the combine: 54 us, 330 TFLOP/s
 // of the definition's products and twice that issued; a tile takes 1300 to 1750 cycles, bound by
@@ -44,10 +46,10 @@ namespace lun {
 
 constexpr int kBlockRows = 128, kBlockThreads = 448, kBlockStages = 6;
 constexpr float kBlockShift = 7.0f, kBlockRaise = 8.0f;
-constexpr int kBlockDrain = 8;
 
 template <int D> struct Kv4BlockLayout {
     static constexpr int half = Kv4Layout<D>::block / 2;
+    static constexpr int drain(int parts) { return parts == 2 ? 4 : 8; }  // tiles that O sums up on the tensor cores
     static constexpr int tile = kPage * D * 2;                 // 64 keys of K, or of V, in FP16
     static constexpr int k_tiles = 0, v_tiles = 4 * tile;      // two buffers of two tiles, and of one
     static constexpr int k_ring = 6 * tile, v_ring = k_ring + kBlockStages * half;
@@ -326,7 +328,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
 #pragma unroll
                     for (int part = 0; part < 2; part++)
                         tc_mma_f16_tmem_a(tmem + o_col, pa + 32u * part + 8u * ks, v + (ks * 2048 >> 4), idesc_o,
-                                          ks || part || (parts == 2 ? j % kBlockDrain != 0 : j > 0));
+                                          ks || part || j % B::drain(parts) != 0);
                 tc_commit(&v_free[b]);
                 tc_commit(&o_done[b]);
             }
@@ -478,8 +480,9 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             if (lane == 0) mbar_arrive(q_ready);
         }
         const int all_see = first_position + t0;  // every live row sees keys up to here
-        float m = -INFINITY, l = 0.0f;
-        // FP32: what O held every kBlockDrain tiles, and what has scaled it since; where q's row was
+        // l_rest: what the additions to l have rounded off, which would add up over thousands of tiles
+        float m = -INFINITY, l = 0.0f, l_rest = 0.0f;
+        // what O held every few tiles, and what has scaled it since; where q's row was
         float4 *drained = reinterpret_cast<float4 *>(base + B::q_rows + row * B::q_stride);
         float since = 1.0f;
         bool ok = true;
@@ -510,40 +513,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             const bool raise = m != -INFINITY && (mx - m) * back > kBlockRaise;
             const float corr = raise ? exp2_fast((m - mx) * back) : 1.0f;
             if (m == -INFINITY || raise) m = mx;
-            if (parts == 2 && j > 0 && j % kBlockDrain == 0) {
-                // P V of the tile before has landed, and P V of this one starts from zero
-                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(lane_base + o_col + c, o);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        float4 sum = j == kBlockDrain ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : drained[(c + i) / 4];
-                        sum.x = fmaf(sum.x, since, __uint_as_float(o[i]));
-                        sum.y = fmaf(sum.y, since, __uint_as_float(o[i + 1]));
-                        sum.z = fmaf(sum.z, since, __uint_as_float(o[i + 2]));
-                        sum.w = fmaf(sum.w, since, __uint_as_float(o[i + 3]));
-                        drained[(c + i) / 4] = sum;
-                    }
-                }
-                since = corr;
-            } else if (__any_sync(0xffffffffu, raise)) {
-                // O's row *= corr once P V of the tile before has landed
-                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(lane_base + o_col + c, o);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                    tmem_st32(lane_base + o_col + c, o);
-                }
-                since *= corr;
-            }
             l *= corr;
+            l_rest *= corr;
             const float zero = m == -INFINITY ? 0.0f : -m;
             uint64_t sum = pack2(0.0f, 0.0f);
             const uint64_t back2 = pack2(back, back), zero2 = pack2(zero, zero), shift2 = pack2(kBlockShift, kBlockShift);
@@ -566,7 +537,44 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             }
             float sum0, sum1;
             unpack2(sum, sum0, sum1);
-            l += sum0 + sum1;
+            sum0 += sum1;
+            const float l_next = l + sum0;
+            l_rest += sum0 - (l_next - l);
+            l = l_next;
+            // with this tile's weights done, so that P V of the tile before has mostly landed
+            if (j > 0 && j % B::drain(parts) == 0) {
+                // P V of the tile before has landed, and P V of this one starts from zero
+                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(lane_base + o_col + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 sum = j == B::drain(parts) ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : drained[(c + i) / 4];
+                        sum.x = fmaf(sum.x, since, __uint_as_float(o[i]));
+                        sum.y = fmaf(sum.y, since, __uint_as_float(o[i + 1]));
+                        sum.z = fmaf(sum.z, since, __uint_as_float(o[i + 2]));
+                        sum.w = fmaf(sum.w, since, __uint_as_float(o[i + 3]));
+                        drained[(c + i) / 4] = sum;
+                    }
+                }
+                since = corr;
+            } else if (__any_sync(0xffffffffu, raise)) {
+                // O's row *= corr once P V of the tile before has landed
+                if (!(ok = kv4_warp_wait(&o_done[(j - 1) & 1], (j - 1) >> 1 & 1, abort_word))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(lane_base + o_col + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                    tmem_st32(lane_base + o_col + c, o);
+                }
+                since *= corr;
+            }
             tmem_st32(lane_base + sb, ph);
             tmem_st32(lane_base + sb + 32u, pl);
             tc_fence_before();
@@ -581,6 +589,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (__all_sync(0xffffffffu, ok && !*abort_word)) {
             tc_fence_after();
+            l += l_rest;
             const bool whole = p.splits == 1;
             const float inverse = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
             T *out = static_cast<T *>(p.out) + tensor_row * p.out_stride + (size_t)(live ? head : 0) * D;
@@ -596,7 +605,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                     for (int i = 0; i < 32; i++) o[i] = 0u;
                 }
                 if (!live) continue;
-                if (parts == 2 && tiles > kBlockDrain) {
+                if (tiles > B::drain(parts)) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 sum = drained[(c + i) / 4];

@@ -118,7 +118,10 @@ WALKS = [  # type, dim, kv heads, group, counts, pages of a sequence
     ("f32", 64, 256, 1, [1] * 40, 40),       # shares of several whole items
     ("bf16", 128, 8, 8, [1] * 64, 2048),
     ("f16", 128, 8, 4, [1] * 64, 2048),
-    ("f16", 64, 16, 16, [1] * 30, 1500)]
+    ("f16", 64, 16, 16, [1] * 30, 1500),
+    ("f32", 128, 4, 4, [32] * 37, 500),      # blocks of rows, 148 of them
+    ("f16", 128, 4, 4, [32] * 37, 2048),
+    ("bf16", 64, 4, 4, [32] * 37, 300)]
 
 
 @pytest.mark.parametrize("name,dim,heads,group,counts,pages", WALKS)
