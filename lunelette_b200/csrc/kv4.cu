@@ -301,6 +301,7 @@ static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_
     cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kListWarps>>(smem);
     if (e != cudaSuccess) return e;
     p.items = reinterpret_cast<int2 *>(reinterpret_cast<char *>(p.part) + a.items_offset);
+    p.list_warps = a.ctas * kListWarps;
     const size_t pages = (size_t)p.rows.max_length / kPage + 1;
     if (a.items > (size_t)INT_MAX / 64 || a.items * pages > (size_t)INT_MAX) return cudaErrorInvalidValue;
     e = launch(kv4_decode_kernel<D, T, NT, kListWarps>, dim3((unsigned)a.ctas), dim3(32 * kListWarps), smem, stream, p);

@@ -75,7 +75,8 @@ struct Kv4AttnParams {
     // unnormalised o, m, l, D + 2 floats a row: [2 warp + (0 the warp's first item, 1 its last)][row of
     // the tile] of the decode kernel, [row][query head][split] of the block kernel
     float *part;
-    int2 *items;  // decode kernel: an item's first part (-1: it is written out) and last warp
+    int2 *items;     // decode kernel: an item's first part (-1: it is written out) and last warp
+    int list_warps;  // and the warps of the list
     int *status;
 };
 
@@ -986,6 +987,13 @@ __device__ __forceinline__ void kv4_combine(const Kv4AttnParams &p, At &&at, int
     for (int e = 0; e < per; e++) dst[e] = from_float<T>(x[e] * inverse);
 }
 
+// Whether an item's record names parts of the list's warps. A warp that gave up a wait leaves its items'
+// records as the workspace had them, which is no content at all.
+__host__ __device__ inline bool kv4_valid_record(int first_part, int last_warp, int list_warps)
+{
+    return first_part >= 0 && last_warp < list_warps && last_warp >= first_part >> 1;
+}
+
 // The decode kernel's rows, [item][row of the tile], a block each, of 4 warps, or 8 where
 // items have many parts (64 sequences of up to 4352 keys, decode and combine together: 42.2
 // us, with 2 warps 43.4, with 1 45.0; 4 of 8000 keys: 24.0 with 8, 26.5 by one warp that
@@ -1003,8 +1011,14 @@ static __global__ void __launch_bounds__(32 * Warps) kv4_combine_kernel(Kv4AttnP
     const Kv4Sequence q = kv4_sequence(p.rows, s);
     if (!q.ok || q.count * p.group > p.most || r >= q.count * p.group) return;
     const int token = r / p.group, head = kvh * p.group + r - token * p.group;
-    if (q.length <= 0) where = make_int2(0, -1);  // no keys: no parts
-    else if (where.x < 0) return;
+    if (q.length <= 0) {
+        where = make_int2(0, -1);  // no keys: no parts
+    } else if (where.x == -1) {
+        return;
+    } else if (!kv4_valid_record(where.x, where.y, p.list_warps)) {
+        if (threadIdx.x == 0) kv4_report(p.status, kKv4Timeout);
+        return;
+    }
     // the first part, then the first of each warp up to the last
     const float *part = p.part + (size_t)(r - r0) * (D + 2);
     const int first_warp = where.x >> 1;
