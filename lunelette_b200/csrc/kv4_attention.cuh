@@ -103,6 +103,17 @@ __device__ __forceinline__ bool kv4_warp_wait(uint64_t *bar, unsigned parity, vo
     return __all_sync(0xffffffffu, kv4_wait(bar, parity, abort_word));
 }
 
+// What this CTA has in flight once a wait gave up: the abort word does not end this wait, half a
+// millisecond does.
+__device__ __forceinline__ bool kv4_landed(uint64_t *bar, unsigned parity)
+{
+    for (unsigned spin = 0; spin < 1024; spin++) {
+        if (mbar_test_wait(bar, parity)) return true;
+        __nanosleep(500);
+    }
+    return false;
+}
+
 // The softmax's weights are taken times 2^14, and l with them: the largest is
 // 16384, and the FP16 parts of a weight keep 22 bits down to 2^-28 of it, where a
 // largest weight of 1 would leave small ones on the 2^-24 grid of FP16's
@@ -800,8 +811,7 @@ static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? 
     }
     if (!ok) {
         // copies may be in flight: see them land (bounded) before the CTA's memory goes
-        for (int i = 0; i < SLOTS; i++)
-            for (unsigned spin = 0; spin < 1024 && !mbar_test_wait(&bar[i], phases >> i & 1); spin++) __nanosleep(500);
+        for (int i = 0; i < SLOTS; i++) kv4_landed(&bar[i], phases >> i & 1);
     }
     __syncthreads();
     if (*abort_word && threadIdx.x == 0) kv4_report(p.status, kKv4Timeout);

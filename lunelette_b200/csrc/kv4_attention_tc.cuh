@@ -167,7 +167,8 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
     uint64_t *k_ready = tiles_at, *k_free = tiles_at + 2, *v_ready = tiles_at + 4, *v_free = tiles_at + 6;  // FP16 tiles
     uint64_t *s_full = tiles_at + 8, *p_ready = tiles_at + 10, *o_done = tiles_at + 12, *q_ready = tiles_at + 14;
     uint64_t *q_full = tiles_at + 15;  // rows of q staged, a barrier a warp
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 19);
+    uint64_t *products_done = tiles_at + 19;  // all of them
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tiles_at + 20);
     volatile int *abort_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *where = reinterpret_cast<int *>(tmem_slot + 2);    // sequence, place
     int *poison = where + 2;                                // per group of dims: first position with a NaN value
@@ -214,6 +215,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         }
         mbar_init(q_ready, 4);
         for (int i = 0; i < 4; i++) mbar_init(&q_full[i], 1);
+        mbar_init(products_done, 1);
         *abort_word = 0;
         for (int i = 0; i < 4; i++) poison[i] = 0x7fffffff;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -277,9 +279,9 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
         // every copy issued has landed before the CTA ends
         if (lane == 0) {
             for (int j = max(0, ik - N); j < ik; j++)
-                kv4_wait(&k_full[j % N], (j / N) & 1, abort_word);
+                if (!kv4_wait(&k_full[j % N], (j / N) & 1, abort_word)) kv4_landed(&k_full[j % N], (j / N) & 1);
             for (int j = max(0, iv - N); j < iv; j++)
-                kv4_wait(&v_full[j % N], (j / N) & 1, abort_word);
+                if (!kv4_wait(&v_full[j % N], (j / N) & 1, abort_word)) kv4_landed(&v_full[j % N], (j / N) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -334,6 +336,10 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
             }
             __syncwarp();
         }
+        // every product issued has ended before tensor memory and the tiles go
+        if (leader) tc_commit(products_done);
+        __syncwarp();
+        if (!kv4_warp_wait(products_done, 0, abort_word)) kv4_landed(products_done, 0);
     } else if (warp < 6) {
         // ---- K: a unit is 16 (8 for 64 dims) bytes of a key's row, word j of them is word 4 j + t of the
         // row; keys k and k + 4 share a quarter warp, whose stores then hit every bank once
@@ -440,7 +446,7 @@ static __global__ void __launch_bounds__(kBlockThreads, 1) kv4_block_kernel(Kv4A
                 if (lane == 0) mbar_expect_tx(full, rows_live * (unsigned)(D * sizeof(T)));
                 __syncwarp();
                 if (live) bulk_g2s(mine + lane * B::q_stride, src, D * sizeof(T), full);
-                landed = kv4_warp_wait(full, 0, abort_word);
+                if (!(landed = kv4_warp_wait(full, 0, abort_word))) kv4_landed(full, 0);
             } else {
                 for (int d = 0; d < D; d++) reinterpret_cast<T *>(mine + lane * B::q_stride)[d] = src[d];
                 __syncwarp();

@@ -37,3 +37,28 @@ def test_records_that_are_followed_stay_among_the_parts(guards):
                     assert all(0 <= p < 2 * warps for p in parts) and 1 <= last - (first >> 1) + 1 <= warps
                 if 0 <= first < 2 * warps and (first >> 1) <= last < warps:
                     assert ok
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aborted", [0, 1])
+def test_waits_end_and_copies_in_flight_are_seen_to_land(guards, aborted):
+    """A barrier that nothing completes: a wait ends after a second, or soon once another warp gave up. What is
+    in flight is waited for all the same, and that wait ends too."""
+    import torch
+
+    class Waits(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_int) for n in ("waited", "landed", "copied", "abort_word")] + [
+            ("wait_ns", ctypes.c_ulonglong), ("land_ns", ctypes.c_ulonglong), ("words_right", ctypes.c_int)]
+
+    src = torch.arange(1024, dtype=torch.int32, device="cuda")
+    out = torch.zeros(ctypes.sizeof(Waits), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert guards.run_waits(ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(src.data_ptr()), aborted) == 0
+    got = Waits.from_buffer_copy(out.cpu().numpy().tobytes())
+    assert got.copied and got.words_right == 1024
+    assert not got.waited and got.abort_word == 1
+    if aborted:
+        assert got.wait_ns < 5e8
+    else:
+        assert 0.99e9 < got.wait_ns < 2e9
+    assert not got.landed and got.land_ns < 1e8
