@@ -105,6 +105,13 @@ int block_rows_for(size_t rows, unsigned threads)
 
 unsigned threads_for(size_t work, size_t most) { return (unsigned)(work < most ? (work + 31) / 32 * 32 : most); }
 
+// Blocks of a call over rows: for the rows, and with a status word to look at the sequences.
+dim3 grid_for(const lunelette_cuda_rows *rows, int block_rows, unsigned threads, const int *status)
+{
+    const size_t checks = status ? (rows->sequences + threads - 1) / threads : 0;
+    return dim3((unsigned)((rows->rows + block_rows - 1) / block_rows + (checks < 148 ? checks : 148)));
+}
+
 int ok(cudaError_t e) { return e == cudaSuccess ? 0 : -1; }
 
 }  // namespace
@@ -155,7 +162,7 @@ LUN_API int lunelette_cuda_kv4_append(const lunelette_cuda_kv4 *cache, size_t la
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
         auto kernel = cache->head_dim == 128 ? kv4_append_kernel<128, T> : kv4_append_kernel<64, T>;
-        return launch(kernel, dim3((unsigned)((rows->rows + p.block_rows - 1) / p.block_rows)), dim3(threads), 0, (cudaStream_t)stream, p);
+        return launch(kernel, grid_for(rows, p.block_rows, threads, status), dim3(threads), 0, (cudaStream_t)stream, p);
     }));
 }
 
@@ -185,7 +192,7 @@ LUN_API int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t laye
     return ok(by_type(type, [&](auto t) {
         using T = decltype(t);
         auto kernel = cache->head_dim == 128 ? kv4_read_kernel<128, T> : kv4_read_kernel<64, T>;
-        return launch(kernel, dim3((unsigned)((rows->rows + p.block_rows - 1) / p.block_rows)), dim3(threads), 0, (cudaStream_t)stream, p);
+        return launch(kernel, grid_for(rows, p.block_rows, threads, status), dim3(threads), 0, (cudaStream_t)stream, p);
     }));
 }
 

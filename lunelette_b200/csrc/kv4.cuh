@@ -119,11 +119,10 @@ constexpr int kKv4BlockRows = 8;
 struct Kv4Place {
     int position, page;
 };
-__device__ __forceinline__ int kv4_position(const Kv4Rows &r, int row, int *status, const int *&table)
+__device__ __forceinline__ int kv4_position(const Kv4Rows &r, int row, const int *&table)
 {
     int s;
     const Kv4Sequence q = kv4_sequence_of_row(r, row, s);
-    if (!q.ok && status && (threadIdx.x & 31) == 0) kv4_report(status, kKv4BadRows);
     table = r.page_tables + s * r.table_stride;
     const bool in = q.ok && row >= q.first && row < q.first + q.count;
     return in ? max(-1, q.length - q.count + (row - q.first)) : -1;
@@ -137,14 +136,14 @@ __device__ __forceinline__ Kv4Place kv4_places(const Kv4Rows &r, int pages, int 
     const int *table;
     if (n == 1) {
         Kv4Place place;
-        place.position = kv4_position(r, row0, threadIdx.x == 0 ? status : nullptr, table);
+        place.position = kv4_position(r, row0, table);
         place.page = place.position >= 0 ? table[place.position / kPage] : 0;
         return place;
     }
     int mine = -1;
     const int *my_table = nullptr;
     for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5) {
-        const int position = kv4_position(r, row0 + i, status, table);
+        const int position = kv4_position(r, row0 + i, table);
         if (lane == 0) places[i].position = position;
         if (lane == i / (blockDim.x >> 5)) mine = position, my_table = table;
     }
@@ -155,6 +154,16 @@ __device__ __forceinline__ Kv4Place kv4_places(const Kv4Rows &r, int pages, int 
         if ((unsigned)page >= (unsigned)pages) kv4_report(status, kKv4BadPage);
     }
     return places[0];
+}
+// The blocks behind those of the rows look at every sequence, for no row falls in one whose offsets
+// descend, or in an empty one. True in such a block, which is done then.
+__device__ __forceinline__ bool kv4_check_sequences(const Kv4Rows &r, int block_rows, int *status)
+{
+    const int row_blocks = (r.rows + block_rows - 1) / block_rows, check = (int)blockIdx.x - row_blocks;
+    if (check < 0) return false;
+    for (int s = check * blockDim.x + threadIdx.x; s < r.sequences; s += ((int)gridDim.x - row_blocks) * blockDim.x)
+        if (!kv4_sequence(r, s).ok) kv4_report(status, kKv4BadRows);
+    return true;
 }
 __device__ __forceinline__ void kv4_check_page(const Kv4Place &place, int pages, int *status)
 {
@@ -365,6 +374,7 @@ static __global__ void __launch_bounds__(512, 2) kv4_append_kernel(Kv4AppendPara
     const int row0 = blockIdx.x * p.block_rows, n = min(p.block_rows, p.rows.rows - row0);
     pdl_wait();
     pdl_launch_dependents();
+    if (kv4_check_sequences(p.rows, p.block_rows, p.status)) return;
     // K heads, V heads, query heads: a thread's values are h = its first head, h + step, ..., row after row
     Raw8<T> raw_lo, raw_hi;
     auto values = [&](int r, int h) {
@@ -496,6 +506,7 @@ static __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4ReadParams p)
     const int row0 = blockIdx.x * p.block_rows, n = min(p.block_rows, p.rows.rows - row0);
     pdl_wait();
     pdl_launch_dependents();
+    if (kv4_check_sequences(p.rows, p.block_rows, p.status)) return;
     const Kv4Place first = kv4_places(p.rows, p.cache.pages, row0, n, places, p.status);
     if (n == 1) kv4_check_page(first, p.cache.pages, p.status);
     else __syncthreads();

@@ -138,3 +138,21 @@ def test_long_walks_keep_their_accuracy(torch, name, dim, heads, group, counts, 
         half = half_step(torch, name)
         bound = half * want.abs() + (1 + half) * size * e + (2.0 ** -25 if name == "f16" else 0.0)
         assert (error / bound).max().item() <= 1.0
+
+
+def test_append_and_read_report_every_broken_sequence(torch):  # noqa: F811
+    """Sequences that no row's search lands on: one whose offsets descend among others within their bounds,
+    and an empty one with a length past the bound, the last of many."""
+    for offsets, lengths, bit in (([0, 3, 2, 5], [3, 9, 3], 1), ([0, 2, 2, 4], [2, 129, 2], 1), ([0, 2, 2, 4], [2, 128, 2], 0),
+                                  ([0] * 4001 + [2], [1] * 4000 + [2], 0), ([0] * 4001 + [2], [1] * 3999 + [-1, 2], 1)):
+        n = len(lengths)
+        c = Cache(torch, [1] * n, [1] * n, 1, 64, max_count=3, max_length=128, stride=2)
+        c.rows = 5 if n == 3 else 2
+        c.d_offsets.copy_(torch.tensor(offsets, dtype=torch.int32))
+        c.d_lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        x = torch.ones((c.rows, 64), device="cuda")
+        c.append("f32", x, x)
+        assert c.status.item() == bit, (offsets[:5], "append")
+        c.status.zero_()
+        c.read("f32", x, None)
+        assert c.status.item() == bit, (offsets[:5], "read")
