@@ -265,8 +265,10 @@ int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t layer, const
  * content expected or kept) holds at least
  * lunelette_cuda_kv4_attention_workspace() bytes for the same sizes; calls that
  * may overlap on the GPU, captured graphs among them, need one each. The bounds'
- * sequences * kv_heads * row tiles * pages stay below 2^31. A deterministic
- * result: the same call gives the same bits. */
+ * sequences * kv_heads * row tiles * pages stay below 2^31, and where a block of
+ * more than 16 rows a KV head is split along its keys, rows * query_heads below 2^33
+ * (else -1, before anything is launched). A deterministic result: the same call gives
+ * the same bits. */
 size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows,
     size_t query_heads);
 int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t layer, const lunelette_cuda_rows *rows,

@@ -211,7 +211,9 @@ struct AttnPlan {
     size_t items, items_offset;
     // block kernel
     int least, block_tiles, block_split_pages, block_splits;
+    size_t block_ctas, block_combines;
     size_t part_bytes;
+    bool fits;  // all grids and the list's count of pages
 };
 
 static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_cuda_rows *rows, size_t query_heads,
@@ -219,6 +221,7 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
 {
     AttnPlan a;
     memset(&a, 0, sizeof a);
+    a.fits = true;
     const size_t group = query_heads / cache->kv_heads, part = (cache->head_dim + 2) * sizeof(float);
     const size_t pages = (rows->max_length + kPage - 1) / kPage;
     size_t most = rows->max_count * group;
@@ -252,6 +255,7 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
             a.many_parts = (size_t)a.ctas > 4 * a.items;
             a.items_offset = 2 * (size_t)a.ctas * kListWarps * a.tile_rows * part;
             a.part_bytes = a.items_offset + a.items * sizeof(int2);
+            a.fits = a.items <= INT_MAX / 64 && a.items * (rows->max_length / kPage + 1) <= INT_MAX;
         }
     }
     if (a.block) {
@@ -269,6 +273,9 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
         }
         if (a.block_split_pages < 1) a.block_split_pages = 1;
         if (a.block_splits > 1) a.block_splits = (int)((pages + a.block_split_pages - 1) / a.block_split_pages);
+        a.block_ctas = ctas * a.block_splits;
+        a.block_combines = a.block_splits > 1 ? rows->rows * ((query_heads + 3) / 4) : 0;
+        a.fits = a.fits && a.block_ctas <= INT_MAX && a.block_combines <= INT_MAX;
         const size_t bytes = a.block_splits > 1 ? rows->rows * query_heads * a.block_splits * part : 0;
         if (bytes > a.part_bytes) a.part_bytes = bytes;  // the kernels run one after the other
     }
@@ -309,8 +316,6 @@ static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_
     if (e != cudaSuccess) return e;
     p.items = reinterpret_cast<int2 *>(reinterpret_cast<char *>(p.part) + a.items_offset);
     p.list_warps = a.ctas * kListWarps;
-    const size_t pages = (size_t)p.rows.max_length / kPage + 1;
-    if (a.items > (size_t)INT_MAX / 64 || a.items * pages > (size_t)INT_MAX) return cudaErrorInvalidValue;
     e = launch(kv4_decode_kernel<D, T, NT, kListWarps>, dim3((unsigned)a.ctas), dim3(32 * kListWarps), smem, stream, p);
     if (e != cudaSuccess) return e;
     const unsigned rows = (unsigned)(a.items * a.tile_rows);
@@ -328,12 +333,9 @@ static cudaError_t launch_block(Kv4AttnParams p, const AttnPlan &a, cudaStream_t
     p.split_pages = a.block_split_pages;
     p.splits = a.block_splits;
     p.tiles = a.block_tiles;
-    const size_t ctas = (size_t)a.block_tiles * p.cache.heads * a.block_splits;
-    const size_t combines = (size_t)p.rows.rows * ((p.cache.heads * p.group + 3) / 4);
-    if (ctas > INT_MAX || combines > INT_MAX) return cudaErrorInvalidValue;
-    e = launch(kernel, dim3((unsigned)ctas), dim3(kBlockThreads), smem, stream, p, a.least);
+    e = launch(kernel, dim3((unsigned)a.block_ctas), dim3(kBlockThreads), smem, stream, p, a.least);
     if (e != cudaSuccess || a.block_splits == 1) return e;
-    return launch(kv4_block_combine_kernel<D, T>, dim3((unsigned)combines), dim3(128), 0, stream, p, a.least);
+    return launch(kv4_block_combine_kernel<D, T>, dim3((unsigned)a.block_combines), dim3(128), 0, stream, p, a.least);
 }
 
 template <int D, typename T>
@@ -359,7 +361,7 @@ LUN_API int lunelette_cuda_kv4_attention(const lunelette_cuda_kv4 *cache, size_t
         return -1;
     if (empty) return 0;
     const AttnPlan a = plan_attention(cache, rows, query_heads, type);
-    if (workspace_bytes < a.part_bytes || (a.part_bytes && !workspace)) return -1;
+    if (!a.fits || workspace_bytes < a.part_bytes || (a.part_bytes && !workspace)) return -1;
     Kv4AttnParams p;
     memset(&p, 0, sizeof p);
     p.cache = cache_of(cache, layer);

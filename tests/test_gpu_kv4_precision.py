@@ -156,3 +156,19 @@ def test_append_and_read_report_every_broken_sequence(torch):  # noqa: F811
         c.status.zero_()
         c.read("f32", x, None)
         assert c.status.item() == bit, (offsets[:5], "read")
+
+
+def test_a_refused_attention_call_launches_nothing(torch):  # noqa: F811
+    """More padded rows than the join of the splits has blocks for; the first sequence's only row would be
+    written by the kernel for few rows."""
+    heads, dim, query = 256, 64, 4096
+    c = Cache(torch, [1, 0, 0, 0, 0], [1, 1, 1, 1, 1], heads, dim, stride=1000, layers=1, layer=0)
+    c.rows, c.max_count, c.max_length = 1 << 24, 2, 64000
+    q = torch.ones((1, query * dim), device="cuda")
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(1 << 26, dtype=torch.uint8, device="cuda")
+    assert L.library().lunelette_cuda_kv4_attention(
+        c.kv4(), 0, c.descriptor(), L.FLOAT32, q.data_ptr(), q.stride(0), query, 0.1, out.data_ptr(), out.stride(0),
+        ws.data_ptr(), 1 << 60, c.status.data_ptr(), c.stream()) == -1
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
