@@ -172,3 +172,46 @@ def test_a_refused_attention_call_launches_nothing(torch):  # noqa: F811
         ws.data_ptr(), 1 << 60, c.status.data_ptr(), c.stream()) == -1
     torch.cuda.synchronize()
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("heads,counts,lengths", [(8, [1] * 64, [4352] * 64), (8, [256], [4352]),
+                                                  (2, [1, 40, 2, 1, 1, 1], [5000] * 6)])
+def test_a_workspace_that_is_too_small_is_refused(torch, name, heads, counts, lengths):  # noqa: F811
+    group, dim = 4, 128
+    c = Cache(torch, counts, lengths, heads, dim, layers=1, layer=0)
+    c.pool.zero_()
+    query = heads * group
+    need = L.library().lunelette_cuda_kv4_attention_workspace(c.kv4(), c.descriptor(), query)
+    assert need > 1 << 16
+    q = torch.ones((c.rows, query * dim), dtype=getattr(torch, TYPES[name][1]), device="cuda")
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+
+    def call(pointer, size):
+        return L.library().lunelette_cuda_kv4_attention(
+            c.kv4(), 0, c.descriptor(), TYPES[name][0], q.data_ptr(), q.stride(0), query, 0.1, out.data_ptr(),
+            out.stride(0), pointer, size, c.status.data_ptr(), c.stream())
+
+    for pointer, size in ((None, need), (ws.data_ptr(), 0), (ws.data_ptr() + 4, need)):
+        assert call(pointer, size) == -1, (pointer, size)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    # the function goes by the largest of the types: the least that this one takes
+    refused, taken = 0, need
+    while taken - refused > 1:
+        size = (taken + refused) // 2
+        if call(ws.data_ptr(), size) == 0:
+            taken = size
+        else:
+            refused = size
+    torch.cuda.synchronize()
+    assert need // 4 <= taken <= need
+    out.fill_(7.0)
+    ws.fill_(0x5A)
+    assert call(ws.data_ptr(), taken - 1) == -1
+    torch.cuda.synchronize()
+    assert (out == 7.0).all() and (ws == 0x5A).all()
+    assert call(ws.data_ptr(), taken) == 0
+    torch.cuda.synchronize()
+    assert (out == 0.0).all() and (ws[taken:] == 0x5A).all() and c.status.item() == 0
