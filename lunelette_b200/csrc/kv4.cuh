@@ -304,11 +304,12 @@ __device__ __noinline__ uint32_t kv4_quantise_exactly(const double (&r)[8], floa
 }
 
 // x c - y s and y c + x s with one rounding of the products' sum and one of the
-// second product's error: off by 2^-23 of the result at most, whatever cancels.
+// second product's error: off by 2^-23 of the result at most, whatever cancels. An infinite
+// product has no error to take off.
 __device__ __forceinline__ float kv4_turn(float x, float c, float y, float s)
 {
-    const float t = y * s;
-    return fmaf(x, c, -t) - fmaf(y, s, -t);
+    const float t = y * s, error = fmaf(y, s, -t);
+    return fmaf(x, c, -t) - (error == error ? error : 0.0f);
 }
 
 // Eight values of a lane in FP32 -> their word of codes as in 64 bits. Values that are

@@ -215,3 +215,25 @@ def test_a_workspace_that_is_too_small_is_refused(torch, name, heads, counts, le
     assert call(ws.data_ptr(), taken) == 0
     torch.cuda.synchronize()
     assert (out == 0.0).all() and (ws[taken:] == 0x5A).all() and c.status.item() == 0
+def test_rotated_infinities_of_q_are_the_definitions(torch):  # noqa: F811
+    dim, n = 128, 40
+    rng = np.random.default_rng(61)
+    x = rng.standard_normal((n, 2, dim)).astype(np.float32)
+    for row in range(n):
+        x[row, row % 2, rng.integers(dim)] = np.inf * (-1) ** row
+    x[0, 0, 3], x[0, 0, 67] = np.inf, np.inf
+    x[1, 1, 3], x[1, 1, 67] = np.inf, -np.inf
+    angle = np.arange(1, n + 1)[:, None] * 10000.0 ** (-np.arange(0, dim, 2) / dim)  # no sine is zero
+    cos, sin = (np.concatenate([f(angle)] * 2, 1).astype(np.float32) for f in (np.cos, np.sin))
+    tables = torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda()
+    c = Cache(torch, [n], [n], 1, dim)
+    q = torch.from_numpy(x.reshape(n, -1)).cuda()
+    out = torch.zeros_like(q)
+    k = torch.ones((n, dim), device="cuda")
+    c.append("f32", k, k, q, out, 2, tables)
+    got = out.cpu().numpy().reshape(x.shape)
+    with np.errstate(invalid="ignore"):
+        want = np.stack([ref.rotate(x[i], cos[i].astype(np.float64), sin[i].astype(np.float64)) for i in range(n)])
+    assert np.isinf(want).any() and np.isnan(want).any()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isinf(got), np.isinf(want)) and (np.sign(got) == np.sign(want))[np.isinf(want)].all()
