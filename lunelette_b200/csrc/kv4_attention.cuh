@@ -186,15 +186,16 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v)
 __device__ __forceinline__ float low_half(uint32_t v) { return __low2float(*reinterpret_cast<__half2 *>(&v)); }
 __device__ __forceinline__ float high_half(uint32_t v) { return __high2float(*reinterpret_cast<__half2 *>(&v)); }
 
-// 2^-e with 2^e the power of two at or below x's magnitude, e within +-120;
-// 1 for zero, NaN and infinities.
+// 2^-e with 2^e the power of two at or below x, e within +-120; 1 for zero. Of an infinity a NaN,
+// which the whole row becomes: scores that are all -infinity would look like masked ones.
 __device__ __forceinline__ float power_scale(float x, float &back)
 {
     int e = (int)(__float_as_uint(x) >> 23 & 255) - 127;
-    if (x == 0.0f || e == 128) e = 0;
+    const bool infinite = e == 128;
+    if (x == 0.0f || infinite) e = 0;
     e = max(-120, min(120, e));
     back = __uint_as_float((uint32_t)(127 + e) << 23);
-    return __uint_as_float((uint32_t)(127 - e) << 23);
+    return infinite ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
 

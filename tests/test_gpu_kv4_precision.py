@@ -237,3 +237,23 @@ def test_rotated_infinities_of_q_are_the_definitions(torch):  # noqa: F811
     assert np.isinf(want).any() and np.isnan(want).any()
     assert np.array_equal(np.isnan(got), np.isnan(want))
     assert np.array_equal(np.isinf(got), np.isinf(want)) and (np.sign(got) == np.sign(want))[np.isinf(want)].all()
+
+
+def test_a_row_with_an_infinity_has_no_distribution(torch):  # noqa: F811
+    """Keys of one sign and a minus infinity in q: every score is minus infinity, which is not a mask."""
+    for name in TYPES:
+        for counts, lengths in (([1], [100]), ([1] * 40, [900] * 40), ([30], [90])):
+            c = Cache(torch, counts, lengths, 1, 64, seed=60)
+            for s, n in enumerate(lengths):
+                for kind in (0, 1):
+                    codes, d = ref.quantise(np.full((1, 64), 1.0))
+                    for p in range(n):
+                        ref.store(c.host[c.layer], 64, c.table[s, p // 64], p % 64, codes, d, kind)
+            c.pool.copy_(torch.from_numpy(c.host.reshape(-1)))
+            q = torch.ones((c.rows, 2 * 64), dtype=getattr(torch, TYPES[name][1]), device="cuda")
+            q[-1, 70] = -np.inf
+            out = torch.zeros_like(q)
+            c.attend(name, q, 2, 0.1, out)
+            assert out[-1, 64:].isnan().all(), (name, counts)
+            out[-1, 64:] = 1.0
+            assert torch.isfinite(out).all(), (name, counts)
