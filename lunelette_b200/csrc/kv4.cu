@@ -203,6 +203,7 @@ constexpr size_t kBlockLeast = 16;
 // How a call's keys and rows are split over the GPU.
 struct AttnPlan {
     bool decode, block;  // which kernels run
+    bool split;          // decode kernel: hi and lo columns
     // decode kernel: n tiles and rows of a row tile, row tiles of a sequence's KV head, tiles of 16 keys in
     // a unit, blocks, whether items can have many parts
     int nt, tile_rows, tiles, ctas;
@@ -231,7 +232,10 @@ static AttnPlan plan_attention(const lunelette_cuda_kv4 *cache, const lunelette_
     a.least = a.decode ? (int)kBlockLeast : 0;
     if (a.decode) {
         if (a.block) most = kBlockLeast;
-        const int lane = type == LUNELETTE_CUDA_FLOAT32 ? 4 : 8;  // rows of an n tile
+        // rows of an n tile: hi and lo columns for each of 4, or one for each of 8 16-bit rows, whose weights then take
+        // two products (4 FP16 sequences of 131072 keys, 8 KV heads of 4: 125 us for 150)
+        a.split = type == LUNELETTE_CUDA_FLOAT32 || most <= 4;
+        const int lane = a.split ? 4 : 8;
         a.nt = most <= (size_t)lane ? 1 : 2;
         a.tile_rows = lane * a.nt;
         a.tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
@@ -298,25 +302,25 @@ LUN_API size_t lunelette_cuda_kv4_attention_workspace(const lunelette_cuda_kv4 *
     return wide > narrow ? wide : narrow;
 }
 
-template <int D, typename T, int NT>
+template <int D, typename T, int NT, bool S>
 static cudaError_t launch_decode(Kv4AttnParams p, const AttnPlan &a, cudaStream_t stream)
 {
     p.tiles = a.tiles;
     p.most = a.block ? a.least : INT_MAX;
     if (a.ranks) {
-        constexpr int smem = Kv4Decode<D, T, NT, kClusterWarps>::smem;
-        const cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kClusterWarps>>(smem);
+        constexpr int smem = Kv4Decode<D, T, NT, kClusterWarps, S>::smem;
+        const cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kClusterWarps, S>>(smem);
         if (e != cudaSuccess) return e;
         p.ranks = a.ranks;
-        return launch_cluster(kv4_decode_kernel<D, T, NT, kClusterWarps>, dim3((unsigned)(a.items * a.ranks)),
+        return launch_cluster(kv4_decode_kernel<D, T, NT, kClusterWarps, S>, dim3((unsigned)(a.items * a.ranks)),
                               dim3(32 * kClusterWarps), smem, a.ranks, stream, p);
     }
-    constexpr int smem = Kv4Decode<D, T, NT, kListWarps>::smem;
-    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kListWarps>>(smem);
+    constexpr int smem = Kv4Decode<D, T, NT, kListWarps, S>::smem;
+    cudaError_t e = opt_in<kv4_decode_kernel<D, T, NT, kListWarps, S>>(smem);
     if (e != cudaSuccess) return e;
     p.items = reinterpret_cast<int2 *>(reinterpret_cast<char *>(p.part) + a.items_offset);
     p.list_warps = a.ctas * kListWarps;
-    e = launch(kv4_decode_kernel<D, T, NT, kListWarps>, dim3((unsigned)a.ctas), dim3(32 * kListWarps), smem, stream, p);
+    e = launch(kv4_decode_kernel<D, T, NT, kListWarps, S>, dim3((unsigned)a.ctas), dim3(32 * kListWarps), smem, stream, p);
     if (e != cudaSuccess) return e;
     const unsigned rows = (unsigned)(a.items * a.tile_rows);
     if (a.many_parts) return launch(kv4_combine_kernel<D, T, 8>, dim3(rows), dim3(256), 0, stream, p, a.tile_rows);
@@ -342,7 +346,10 @@ template <int D, typename T>
 static cudaError_t launch_attention(const Kv4AttnParams &p, const AttnPlan &a, cudaStream_t stream)
 {
     cudaError_t e = cudaSuccess;
-    if (a.decode) e = a.nt == 1 ? launch_decode<D, T, 1>(p, a, stream) : launch_decode<D, T, 2>(p, a, stream);
+    constexpr bool wide = sizeof(T) == 4;
+    if (a.decode && a.nt == 2) e = launch_decode<D, T, 2, wide>(p, a, stream);
+    else if (a.decode && a.split) e = launch_decode<D, T, 1, true>(p, a, stream);
+    else if (a.decode) e = launch_decode<D, T, 1, wide>(p, a, stream);
     if (e == cudaSuccess && a.block) e = launch_block<D, T>(p, a, stream);
     return e;
 }

@@ -27,10 +27,11 @@
 // decode step has 1 to 16 query rows a KV head, so a tcgen05 tile of 128 rows would be
 // mostly padding, while here the rows sit in the n = 8 side. FP32 rows of q and
 // weights of the softmax enter as FP16 hi + lo parts in neighbouring columns
-// (22 bits together), so one MMA serves 4 rows at FP32 grade. Of 16-bit rows q is one FP16
-// (exact after a power-of-two scaling but for what lies below 2^-24 of the row's largest), 8
-// rows an MMA; their weights are two FP16 all the same, in two MMAs (with one, off by 2^-12,
-// FP16 outputs lost a fifth more than their own rounding does).
+// (22 bits together), so one MMA serves 4 rows at FP32 grade. Up to 4
+// rows of 16 bits go the same way. More of them have q in one FP16 (exact after a power-of-two
+// scaling but for what lies below 2^-24 of the row's largest), 8 rows an MMA, and their weights in two
+// FP16 all the same, in two MMAs (with one, off by 2^-12, FP16 outputs lost a fifth more than
+// their own rounding does).
 //   S = K Q^T     A: 16 keys x 16 dims of c - 8 (an AND and a subtraction); a group's sum, in FP32, is
 //                 scaled by d after its two MMAs. Codes as they are, with -8 sum q to start a sum
 //                 from, take as long and lose six times as much: the tensor core cuts sums to FP32
@@ -123,13 +124,13 @@ constexpr float kWeightShift = 14.0f, kValueShift = 9.0f, kValueScale = 512.0f;
 constexpr int kListWarps = 4, kListSlots = 3, kListCtas = 4;  // of a block; of a warp; of an SM
 constexpr int kClusterWarps = 8, kClusterSlots = 4, kClusterRanks = 8;  // of a block; of a warp; blocks at most
 
-template <int D, typename T, int NT, int W> struct Kv4Decode {
-    static constexpr bool split = sizeof(T) == 4;    // hi and lo columns
+template <int D, typename T, int NT, int W, bool S> struct Kv4Decode {
+    static constexpr bool split = S;                 // hi and lo columns
     static constexpr int lane_rows = split ? 1 : 2;  // query rows of a lane and n tile
     static constexpr int rows = 4 * NT * lane_rows;  // query rows of a tile
     static constexpr int keys = W > kListWarps ? 16 : 64;  // of a unit
     static constexpr int slots = W > kListWarps ? kClusterSlots : kListSlots;
-    static constexpr int drain = split ? 4 : 12;  // pages that the list sums up on the tensor cores
+    static constexpr int drain = sizeof(T) == 4 ? 4 : 12;  // pages that the list sums up on the tensor cores
     static constexpr int codes = keys * D / 2;
     static constexpr int half = codes + keys * 2 * (D / 32);  // K or V of a unit, laid out as in a page
     static constexpr int ring = W * slots * half;
@@ -217,13 +218,13 @@ __device__ __forceinline__ Kv4Share kv4_share(const Kv4AttnParams &p, const Kv4S
 
 // Items [sequence][KV head][row tile of p.tiles]. W = kListWarps: any number of blocks
 // share the list. W = kClusterWarps: a cluster per item.
-template <int D, typename T, int NT, int W>
+template <int D, typename T, int NT, int W, bool S>
 static __global__ void __launch_bounds__(32 * W, W > kListWarps ? 1 : NT == 1 ? kListCtas : 2)
     kv4_decode_kernel(Kv4AttnParams p)
 {
     namespace cg = cooperative_groups;
     using L = Kv4Layout<D>;
-    using K = Kv4Decode<D, T, NT, W>;
+    using K = Kv4Decode<D, T, NT, W, S>;
     constexpr int G = L::groups, MT = D / 16, RP = K::lane_rows, SLOTS = K::slots, KT = K::keys / 16;
     constexpr bool cluster = W > kListWarps;
     constexpr int row_bytes = D / 2;
