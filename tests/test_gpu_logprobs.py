@@ -160,3 +160,20 @@ def test_same_bits_every_time_and_in_a_graph(torch):
         graph.replay()
         torch.cuda.synchronize()
         assert all(np.array_equal(a, b.cpu().numpy()) for a, b in zip(first, out))
+
+
+@pytest.mark.parametrize("name,rows,vocab", [("f32", 1, 131072), ("f32", 40, 131072), ("bf16", 3, 50001)])
+@pytest.mark.parametrize("left", [0, 1, 3, 40])
+def test_few_adjacent_tokens_left_by_a_mask(torch, name, rows, vocab, left):
+    """A grammar that allows digits, say: fewer tokens than `top`, next to each other, in rows of many blocks."""
+    x = make(torch, name, rows, vocab, seed=9).clone()
+    keep = x[:, 700:700 + left].clone()
+    x[:] = -np.inf
+    x[:, 700:700 + left] = keep
+    if left:
+        check(torch, name, x, 20)
+    lp, ent, ids, tlp = call(torch, name, x, torch.full((rows,), 700, device="cuda"), 20)
+    order = np.sort(ids, 1)
+    rest = np.arange(20 - min(left, 20))
+    assert (order[:, :rest.size] == rest).all() and ((order[:, rest.size:] >= 700) & (order[:, rest.size:] < 700 + left)).all()
+    assert np.isnan(lp).all() == (left == 0) and np.isfinite(lp).all() == (left > 0)

@@ -212,3 +212,31 @@ def test_quantisation_error_is_at_most_half_a_step_inside_and_one_at_the_far_end
     assert (np.abs(ref.dequantise(codes, d) - r) <= np.abs(d) * (1 + 8 * 2.0 ** -8)).all()
     inside = np.abs(r) <= 7.4 * np.abs(d)
     assert (np.abs(ref.dequantise(codes, d) - r)[inside] <= 0.5 * np.broadcast_to(np.abs(d), r.shape)[inside]).all()
+
+
+def test_values_from_subnormal_codes_are_exact_in_fp16():
+    """The decode kernel's conversion: a code alone in a half's bits 0..3 or 4..7 is the subnormal c 2^-24 or
+    c 2^-20; one multiply-add with d 2^15 or d 2^11 and -d 2^-6 leaves d (c - 8) 2^-9. Every operand and the result
+    is an FP16 for 2^-8 <= |d| < 2; elsewhere c - 8, from a half of 1024 + c or 1024 + 16 c, is multiplied by d."""
+    def exact(x):
+        with np.errstate(over="ignore"):
+            return np.array_equal(x, x.astype(np.float16).astype(np.float64))
+
+    every = (np.arange(128, 256)[:, None] * np.exp2(np.arange(-15.0, -6.0))[None]).reshape(-1)
+    every = np.concatenate([every, -every])[:, None]
+    assert np.abs(every).min() == 2.0 ** -8 and np.abs(every).max() < 2.0
+    c = np.arange(16.0)[None]
+    for shift, factor in ((24, 15), (20, 11)):
+        code = c * 2.0 ** -shift
+        bits = (np.arange(16, dtype=np.uint16) << (24 - shift)).view(np.float16).astype(np.float64)
+        assert np.array_equal(code[0], bits)
+        assert exact(every * 2.0 ** factor) and exact(-every * 2.0 ** -6)
+        value = code * (every * 2.0 ** factor) - every * 2.0 ** -6
+        assert np.array_equal(value, every * (c - 8) * 2.0 ** -9) and exact(value)
+    # just outside: a result below FP16's last step, a factor past its largest value
+    assert not exact(np.array([[129 * 2.0 ** -16]]) * (c - 8) * 2.0 ** -9)
+    assert not exact(np.array([2.0 * 2.0 ** 15]))
+    codes = np.arange(16, dtype=np.uint16)
+    low, high = ((0x6400 | codes << s).astype(np.uint16).view(np.float16).astype(np.float64) for s in (0, 4))
+    assert np.array_equal(low - 1032, codes - 8.0) and np.array_equal(high / 16 - 72, codes - 8.0)
+    assert np.array_equal(np.array([0x6408, 0x2c00, 0xd480], np.uint16).view(np.float16), [1032, 1 / 16, -72])
