@@ -69,14 +69,17 @@ def test_16_bit_rows_are_rounded_once(torch, name, dim, heads, group, counts, le
     assert c.status.item() == 0
 
 
-def walk(torch, name, dim, heads, group, counts, pages, mean, seed):  # noqa: F811
-    """Sequences of `pages` whole pages each, drawn from eight that hold values around `mean`. Returns
-    outputs, their definition in 64 bits and sum p |v|, [rows, heads, group, dim]."""
+def walk(torch, name, dim, heads, group, counts, pages, mean, seed, rise=None):  # noqa: F811
+    """Sequences of `pages` whole pages each, drawn from eight that hold values around `mean`; with `rise`, each
+    of the eight has larger keys than those before, q a mean, and they come in that order. Returns outputs,
+    their definition in 64 bits and sum p |v|, [rows, heads, group, dim]."""
     rng = np.random.default_rng(seed)
     held, few = [], 8
     c = Cache(torch, [0], [64 * few], heads, dim, seed=seed, spare=0, layers=1, layer=0)
     for kind in (0, 1):
         x = rng.standard_normal((64 * few, heads, dim)) * (1.0 if kind == 0 else 0.25) + (0.0 if kind == 0 else mean)
+        if rise and kind == 0:
+            x = x + rise * np.arange(few).repeat(64)[:, None, None]
         codes, d = ref.quantise(x)
         for p in range(64 * few):
             ref.store(c.host[0], dim, p // 64, p % 64, codes[p], d[p], kind)
@@ -84,12 +87,14 @@ def walk(torch, name, dim, heads, group, counts, pages, mean, seed):  # noqa: F8
     c.pool.copy_(torch.from_numpy(c.host.reshape(-1)))
     c.counts, c.lengths, c.stride = list(counts), [64 * pages] * len(counts), pages
     c.table = rng.integers(0, few, (len(counts), pages)).astype(np.int32)
+    if rise:
+        c.table.sort(1)
     c.offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
     c.rows, c.max_count, c.max_length = int(c.offsets[-1]), max(counts), 64 * pages
     c.d_offsets, c.d_table = torch.from_numpy(c.offsets).cuda(), torch.from_numpy(c.table).cuda()
     c.d_lengths = torch.tensor(c.lengths, dtype=torch.int32, device="cuda")
     query, scale = heads * group, dim ** -0.5
-    q = tensor(torch, name, rng.standard_normal((c.rows, query * dim)))
+    q = tensor(torch, name, rng.standard_normal((c.rows, query * dim)) + (0.5 if rise else 0.0))
     out = torch.zeros_like(q)
     c.attend(name, q, query, scale, out)
     assert c.status.item() == 0
@@ -138,6 +143,54 @@ def test_long_walks_keep_their_accuracy(torch, name, dim, heads, group, counts, 
         half = half_step(torch, name)
         bound = half * want.abs() + (1 + half) * size * e + (2.0 ** -25 if name == "f16" else 0.0)
         assert (error / bound).max().item() <= 1.0
+
+
+@pytest.mark.parametrize("name,dim,heads,group,counts,pages", [
+    ("f32", 128, 8, 4, [1] * 64, 68), ("f32", 64, 2, 4, [2] * 5, 2048), ("f16", 128, 8, 3, [1] * 64, 136),
+    ("bf16", 128, 8, 8, [1] * 64, 136), ("f16", 64, 16, 16, [1] * 30, 300), ("f32", 128, 4, 4, [32] * 37, 50),
+    ("f16", 64, 4, 4, [32] * 37, 50)])
+@pytest.mark.parametrize("rise", [0.1, 1.0])
+def test_long_walks_while_the_maximum_rises(torch, name, dim, heads, group, counts, pages, rise):  # noqa: F811
+    """What was taken out of the sums is scaled down with them: eight kinds of pages one after the other, each
+    with larger scores than the last."""
+    got, want, size = walk(torch, name, dim, heads, group, counts, pages, 2.0, seed=pages, rise=rise)
+    # sum |q k| is 128 products of 0.9 and 0.8 + 7 rise on average, times 128^-1/2, and under half as much
+    # again in every row: 2^-21 of it, twice, is what moves a weight at most
+    e = cut(name) + 2.0 ** -20 + 1.5 * (8.2 + 71 * rise) * 2.0 ** -20
+    half = half_step(torch, name) if name != "f32" else 0.0
+    bound = half * want.abs() + (1 + half) * size * e + (2.0 ** -25 if name == "f16" else 0.0)
+    assert ((got - want).abs() / bound).max().item() <= 1.0
+
+
+@pytest.mark.parametrize("name,dim,heads,group,counts,lengths,at", [
+    ("f32", 64, 16, 4, [1] * 30, [2200] * 30, 100), ("f16", 64, 32, 4, [1] * 30, [2600] * 30, 100),
+    ("bf16", 64, 32, 8, [1] * 30, [2600] * 30, 100), ("f16", 128, 2, 8, [1], [300], 100), ("bf16", 128, 1, 2, [2], [70], 69),
+    ("f16", 64, 1, 4, [60], [900], 870), ("bf16", 128, 1, 4, [90], [1300], 64)])
+def test_a_nan_stays_where_it_is_seen(torch, name, dim, heads, group, counts, lengths, at):  # noqa: F811
+    """A NaN in one group of one position's values, pages before the sums are taken out again, and in rows of
+    every kernel: those dims of the rows that see it, and nothing else."""
+    c = Cache(torch, counts, lengths, heads, dim, seed=70, layers=1, layer=0)
+    rng = np.random.default_rng(71)
+    k, v = (ref.quantise(rng.standard_normal((64, heads, dim))) for _ in range(2))
+    for p in range(64):
+        for kind, (codes, d) in ((0, k), (1, v)):
+            ref.store(c.host[0], dim, 0, p, codes[p], d[p], kind)
+    c.host[0, 1:] = c.host[0, :1]
+    for s in range(0, len(counts), 3):
+        codes, d = (x[at % 64].copy() for x in v)
+        d[0, 1] = np.nan
+        ref.store(c.host[0], dim, c.table[s, at // 64], at % 64, codes, d, 1)
+    c.pool.copy_(torch.from_numpy(c.host.reshape(-1)))
+    query = heads * group
+    q = tensor(torch, name, rng.standard_normal((c.rows, query * dim)))
+    out = torch.zeros_like(q)
+    c.attend(name, q, query, dim ** -0.5, out)
+    got = out.double().cpu().numpy().reshape(c.rows, heads, group, dim)
+    bad = np.zeros(got.shape, bool)
+    for row, s, position in c.rows_of():
+        bad[row, 0, :, 32:64] = s % 3 == 0 and position >= at
+    assert np.array_equal(np.isnan(got), bad)
+    assert c.status.item() == 0
 
 
 def test_append_and_read_report_every_broken_sequence(torch):  # noqa: F811
