@@ -226,9 +226,10 @@ size_t lunelette_cuda_kv4_bytes(size_t layers, size_t pages, size_t kv_heads, si
  *   max_length  at least every length, at most table_stride * 64
  * The functions that take a device word `status` (or NULL) OR 1 into it when a
  * sequence breaks these bounds or its offsets descend (its rows are skipped and
- * left as they are), and 2 when a page lies outside the pool (its positions are
- * skipped); attention ORs 4 when a copy or a tensor-core step has not come back
- * for a second, and its outputs are not valid then. Sequences may be empty, and a row before position 0 (n > length)
+ * left as they are; rows that two others then claim are either's), and 2 when a
+ * page lies outside the pool (its positions are skipped); attention ORs 4 when a
+ * copy or a tensor-core step has not come back for a second, and its outputs are
+ * not valid then. Sequences may be empty, and a row before position 0 (n > length)
  * has no position: nothing is stored or read for it. Sequences of one call must
  * not append to the same page. */
 typedef struct lunelette_cuda_rows {
@@ -260,9 +261,14 @@ int lunelette_cuda_kv4_read(const lunelette_cuda_kv4 *cache, size_t layer, const
 /* Causal attention over the cache: row r's query heads (query_heads a multiple
  * of kv_heads, head h over KV head h / (query_heads / kv_heads)) see positions
  * 0..its own of its sequence: out = sum_p softmax_p(scale * q . k_p) v_p, with
- * scores, softmax and sums as in FP32. Rows without a position get zeros. q is
- * rotated already and may not overlap out. `workspace` (16-byte aligned, no
- * content expected or kept) holds at least
+ * scores, softmax and sums as in FP32 whatever `type` is, rounded once at the end.
+ * (Rows of q and the weights enter the tensor cores in FP16 parts that keep 22 bits;
+ * rows of 16 bits keep what is above 2^-24 of their largest element. The tensor
+ * cores cut their sums towards zero: what they add up before it is summed to
+ * nearest loses 1e-6 to 3e-6 of sum p |v| over values of one sign, for 16-bit rows
+ * up to 1e-5, at any length.) Rows without a position get zeros, rows of q with a
+ * NaN or an infinity NaNs. q is rotated already and may not overlap out.
+ * `workspace` (16-byte aligned, no content expected or kept) holds at least
  * lunelette_cuda_kv4_attention_workspace() bytes for the same sizes; calls that
  * may overlap on the GPU, captured graphs among them, need one each. The bounds'
  * sequences * kv_heads * row tiles * pages stay below 2^31, and where a block of

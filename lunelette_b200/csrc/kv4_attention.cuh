@@ -15,13 +15,15 @@
 // or less (one sequence, or short ones), time is what the steps wait for one another:
 // then a cluster of 1 to 8 blocks takes an item, its warps shares of it in 16 keys, and
 // merges it through distributed shared memory, in one launch (one sequence, 8 KV heads
-// of 4 query heads, FP32: 500 keys 7.9 us by clusters, 11.3 by the list; 4096 keys 12.8
-// by either; 8192 keys 17.8 and 13.2). Clusters of 16 do not all find room at once: 23.9
-// us at 4352 keys. Warps of a block: 8, for 16 take 13.3 us there and 9.2 at 512 keys.
-// Blocks of the list: 4 an SM, 3 slots a warp (3 and 4: 136 us for 130 at four sequences of
-// 131072 keys). Those four, BF16, 8 KV heads of 8, take 128 us with the combine, 4.7 TB/s; 64 FP32
-// sequences of up to 4352 keys, 8 KV heads of 4, 42 us, of which 0.23 us an SM and page go to the
-// chains of conversion, product and softmax, 7 to the combine.
+// of 4 query heads, FP32, in a captured graph: 500 keys 7.5 us by clusters, 10.7 by the list; 2000
+// keys 9.7 and 10.3; 4096 keys 12.3 and 10.8; 8192 keys 17.4 and 13.1). Clusters of 16 do not all
+// find room at once. 4 blocks of 16 warps instead of 8 of 8: 8.8 us at 500 keys.
+// Blocks of the list: 4 an SM, 3 slots a warp (3 of 4 slots: 127 us for 126 at four FP32 sequences of
+// 131072 keys, 150 for 152 at those below). Four BF16 sequences of 131072 keys, 8 KV heads of 8, take
+// 152 us with the combine in a captured graph, 4.0 TB/s; 64 FP32 sequences of up to 4352 keys, 8 KV
+// heads of 4, 43 us, 37 of them in this kernel under a profiler, whose SMs are active for three
+// quarters of it and issue in half of the slots: they wait for the chains of conversion, product and
+// softmax.
 //
 // The products run on mma.sync m16n8k16 with FP16 operands and FP32 sums: a
 // decode step has 1 to 16 query rows a KV head, so a tcgen05 tile of 128 rows would be
@@ -74,7 +76,8 @@ struct Kv4AttnParams {
     int split_pages, splits;  // block kernel: pages of a split; splits, 1: the kernel writes the output itself
     bool wide;
     // unnormalised o, m, l, D + 2 floats a row: [2 warp + (0 the warp's first item, 1 its last)][row of
-    // the tile] of the decode kernel, [row][query head][split] of the block kernel
+    // the tile] of the decode kernel, which keeps what it takes out of o there meanwhile, [row][query
+    // head][split] of the block kernel
     float *part;
     int2 *items;     // decode kernel: an item's first part (-1: it is written out) and last warp
     int list_warps;  // and the warps of the list
@@ -148,7 +151,9 @@ __device__ __forceinline__ float exp2_fast(float x)  // 2 ulp; 0 below 2^-126
 }
 
 // Four codes in the bytes' low and high nibbles of both halves -> c - 8 in FP16:
-// a = (nibble 0, nibble 4), b = (nibble 1, nibble 5) of a word.
+// a = (nibble 0, nibble 4), b = (nibble 1, nibble 5) of a word. The step is a published one of 4-bit
+// weights: a nibble put under the exponent of 1024 is 1024 + c, or 1024 + 16 c from the
+// upper one, and one exact operation takes the 1024 off.
 __device__ __forceinline__ uint32_t kv4_low(uint32_t w)
 {
     uint32_t r;
