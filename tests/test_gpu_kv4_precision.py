@@ -211,6 +211,31 @@ def test_append_and_read_report_every_broken_sequence(torch):  # noqa: F811
         assert c.status.item() == bit, (offsets[:5], "read")
 
 
+@pytest.mark.parametrize("name,dim,heads,group,rows,skew", [("f32", 128, 8, 4, 2500, 0), ("bf16", 64, 3, 7, 3000, 1),
+                                                            ("f16", 128, 1, 40, 1300, 0)])
+def test_append_rotates_many_rows_in_place(torch, name, dim, heads, group, rows, skew):  # noqa: F811
+    """Blocks that take several rows, with the next values already loaded when a row is written over."""
+    c = Cache(torch, [rows - 900, 0, 900], [rows, 0, 1000], heads, dim, layers=1, layer=0)
+    query = heads * group
+    rng = np.random.default_rng(80)
+    qkv = tensor(torch, name, rng.standard_normal((rows, (query + 2 * heads) * dim + skew)))[:, skew:]
+    q, k, v = qkv.split([query * dim, heads * dim, heads * dim], 1)
+    angle = np.arange(rows)[:, None] * 10000.0 ** (-np.arange(0, dim, 2) / dim)
+    tables = [torch.from_numpy(np.concatenate([f(angle)] * 2, 1).astype(np.float32)).cuda() for f in (np.cos, np.sin)]
+    out = torch.zeros((rows, query * dim), dtype=q.dtype, device="cuda")
+    c.append(name, k, v, q, out, query, tables)
+    pool, before = c.pool.clone(), k.clone()
+    c.pool.zero_()
+    c.append(name, k, v, q, q, query, tables)
+    assert torch.equal(q, out) and torch.equal(k, before) and c.status.item() == 0
+    held = torch.zeros((rows, heads * dim), dtype=q.dtype, device="cuda")
+    again = torch.zeros_like(held)
+    c.read(name, held, None)
+    c.pool.copy_(pool)
+    c.read(name, again, None)
+    assert torch.equal(held, again)
+
+
 def test_a_refused_attention_call_launches_nothing(torch):  # noqa: F811
     """More padded rows than the join of the splits has blocks for; the first sequence's only row would be
     written by the kernel for few rows."""
